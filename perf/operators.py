@@ -39,31 +39,31 @@ def _linear(name, tokens, inputs, outputs, **more):
 def listed():
     return [
         # one decode step's tokens: nothing but latency
-        _router("route, 64 tokens of decode", "route", 64, 256, 6, dtype="bf16", train=False),
+        _router("route decode 64", "route", 64, 256, 6, dtype="bf16", train=False),
         # a prompt through a router that selects by a corrected sigmoid score, padded rows among it; odd length
-        _router("route, biased sigmoid, 4099", "route", 4099, 256, 8, score="sigmoid", bias=True, scale=2.5,
+        _router("route biased sigmoid 4099", "route", 4099, 256, 8, score="sigmoid", bias=True, scale=2.5,
                 padding=0.1),
         # the balance loss of one micro-batch whose routes another router chose
-        _router("balance, 8192 of 256", "balance", 8192, 256, 8),
+        _router("balance 8192x256", "balance", 8192, 256, 8),
         # the same for a packed batch of ragged sequences, some of them empty, with padding; uneven expert count
-        _router("balance, 13 ragged sequences", "balance", 5003, 160, 6, score="sigmoid", dtype="bf16", padding=0.05,
+        _router("balance 13 ragged sequences", "balance", 5003, 160, 6, score="sigmoid", dtype="bf16", padding=0.05,
                 sequences=13),
         # a training step of the router: headline layer of this repository's benchmark
-        _router("step, 8192 of 256", "step", 8192, 256, 8),
+        _router("step 8192x256", "step", 8192, 256, 8),
         # the largest router step: long batch, many experts, a loss for each of 16 sequences
-        _router("step, 65536 of 512", "step", 65536, 512, 8, score="sigmoid", bias=True, dtype="bf16", sequences=16),
+        _router("step 65536x512", "step", 65536, 512, 8, score="sigmoid", bias=True, dtype="bf16", sequences=16),
         # a dense projection of 64 decode tokens: the weights are read once
-        _matmul("matmul, 64 tokens", 64, 4096, 4096),
+        _matmul("matmul decode 64", 64, 4096, 4096),
         # odd sizes, scales with mantissas as imported checkpoints carry them, FP32 result
-        _matmul("matmul, odd, any scales", 1237, 1000, 1100, mantissas=True, out="fp32"),
+        _matmul("matmul odd any scales", 1237, 1000, 1100, mantissas=True, out="fp32"),
         # a prompt's projection, the largest product
-        _matmul("matmul, 8192 x 4096 x 4096", 8192, 4096, 4096),
+        _matmul("matmul 8192x4096x4096", 8192, 4096, 4096),
         # a weight gradient: both operands in 1 x 128 blocks along the tokens, FP32 result
-        _matmul("matmul, weight gradient", 4096, 2048, 8190, b_block_rows=1, out="fp32"),
+        _matmul("matmul weight gradient", 4096, 2048, 8190, b_block_rows=1, out="fp32"),
         # a projection for one token
-        _linear("linear, one token", 1, 4096, 2048, train=False),
+        _linear("linear one token", 1, 4096, 2048, train=False),
         # forward and backward of a projection over the headline batch
-        _linear("linear, training step, 8192", 8192, 2048, 4096),
+        _linear("linear training step 8192", 8192, 2048, 4096),
     ]
 
 
