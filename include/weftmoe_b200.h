@@ -281,6 +281,56 @@ WM_API int wm_stage_inputs(const void* x, int64_t x_row_stride, const void* ids,
 WM_API int wm_scatter_output(const void* output, int32_t tokens, int32_t start, int32_t valid_rows,
                              int32_t hidden, void* result, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Router operators: the choice of K experts per token with its gates, per-expert counts, and the balance
+ * loss, each with its gradient.  They produce the routes and gates that wm_forward takes and consume the
+ * dgates that wm_backward returns; the reference leaves this step to its host framework.
+ *
+ * logits [tokens][experts], rows row_stride elements apart; -inf = this expert is not available to this token.
+ * score 0: softmax over the available experts; 1: sigmoid.  routes: the top_k largest logits, or, with bias, the
+ * largest score + bias (scores in 64 bits; finite bias), ties to the lowest id, -1 where no expert is left.
+ * gates: scale * score, with renormalize divided by the sum of the chosen scores; 0 where the route is -1.
+ * A token is dead where padding[token] != 0 or, with sequences (offsets [num_sequences + 1], non-decreasing, sequence
+ * b = tokens [sequences[b], sequences[b+1])), where no sequence holds it: routes -1, gates 0, gradient 0, in no
+ * sum, whatever its logits hold.  A live token with a NaN (for softmax also +inf) logit gets the routes
+ * 0..top_k-1 with NaN gates, and NaN gradients.
+ * Balance loss: mean over the sequences that have a live token of sum_e f_e P_e; f_e = experts * counts_e / sum of
+ * counts, P_e = mean over live tokens of score_e / (sum of the token's scores).  Its gradient takes counts as given.
+ * Results do not depend on the order in which blocks run.  No call synchronises or allocates; all may be captured.
+ * experts <= 1024, top_k <= 32, num_sequences <= 65535. */
+typedef struct wm_router {
+  const void* logits;
+  int64_t row_stride;       /* elements, >= experts                                                */
+  int32_t dtype;            /* 0 BF16, 1 FP32, 2 FP16                                              */
+  int32_t tokens;
+  int32_t experts;
+  int32_t top_k;            /* ignored by wm_balance_forward                                       */
+  int32_t score;            /* 0 softmax, 1 sigmoid                                                */
+  int32_t renormalize;
+  float scale;              /* finite, positive                                                    */
+  int32_t num_sequences;    /* 0 without offsets: the batch is one sequence                        */
+  const float* bias;        /* [experts] or NULL                                                   */
+  const uint8_t* padding;   /* [tokens] or NULL                                                    */
+  const int32_t* sequences; /* [num_sequences + 1] or NULL                                         */
+} wm_router;
+/* Bytes of the workspace of a forward call that computes the loss. */
+WM_API int wm_router_workspace(const wm_router* router, int64_t* bytes);
+/* routes / gates [tokens][top_k].  counts, loss, table and workspace are NULL together (no loss), or:
+ * counts [max(1, num_sequences)][experts], loss [1], table [max(1, num_sequences) * experts + 1] FP32, which the
+ * backward call reads.  The workspace is free again when the call's kernels are done. */
+WM_API int wm_router_forward(const wm_router* router, int32_t* routes, float* gates, int32_t* counts, float* loss,
+                             float* table, void* workspace, int64_t workspace_bytes, void* stream);
+/* The loss for given counts (another router's, or summed over ranks). */
+WM_API int wm_balance_forward(const wm_router* router, const int32_t* counts, float* loss, float* table,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+/* dlogits [tokens][experts] contiguous, of the logits' type: the gates' part (routes, dgates [tokens][top_k]), the
+ * loss's part (table, dloss [1] on the device), or both added in FP32; the absent pair is NULL. */
+WM_API int wm_router_backward(const wm_router* router, const int32_t* routes, const float* dgates,
+                              const float* table, const float* dloss, void* dlogits, void* stream);
+/* counts [max(1, num_sequences)][experts] = routes per expert; ids outside [0, experts) count nowhere. */
+WM_API int wm_expert_counts(const int32_t* routes, int32_t tokens, int32_t top_k, int32_t experts,
+                            const int32_t* sequences, int32_t num_sequences, int32_t* counts, void* stream);
+
 /* Diagnostic: one grouped GEMM on caller buffers (synchronises `stream`).
  * kind 0: out[rows,n]   = a[rows,k] * b[g][n,k]^T          (FC2 form)
  * kind 1: out[rows,n]   = a[rows,k] * b[g][k,n]            (dU / dX form)

@@ -41,6 +41,13 @@ class WmRouteOut(Structure):
         "padded_rows", "dst_primary")]
 
 
+class WmRouter(Structure):
+    _fields_ = [("logits", c_void_p), ("row_stride", c_int64), ("dtype", c_int32), ("tokens", c_int32),
+                ("experts", c_int32), ("top_k", c_int32), ("score", c_int32), ("renormalize", c_int32),
+                ("scale", c_float), ("num_sequences", c_int32), ("bias", c_void_p), ("padding", c_void_p),
+                ("sequences", c_void_p)]
+
+
 # name -> (restype, argtypes); every entry is declared in include/weftmoe_b200.h
 SIGNATURES = {
     "wm_last_error": (c_char_p, []),
@@ -76,6 +83,11 @@ SIGNATURES = {
     "wm_stage_inputs": (c_int, [c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64] + [c_int32] * 5
                         + [c_void_p, c_void_p, c_void_p, c_void_p]),
     "wm_scatter_output": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "wm_router_workspace": (c_int, [POINTER(WmRouter), POINTER(c_int64)]),
+    "wm_router_forward": (c_int, [POINTER(WmRouter)] + [c_void_p] * 6 + [c_int64, c_void_p]),
+    "wm_balance_forward": (c_int, [POINTER(WmRouter)] + [c_void_p] * 4 + [c_int64, c_void_p]),
+    "wm_router_backward": (c_int, [POINTER(WmRouter)] + [c_void_p] * 6),
+    "wm_expert_counts": (c_int, [c_void_p] + [c_int32] * 3 + [c_void_p, c_int32, c_void_p, c_void_p]),
     "wm_debug_force_gemm_pairs": (None, [c_int]),
     "wm_debug_set_wait_budget": (c_int, [ctypes.c_longlong]),
     "wm_debug_wait_flag": (c_int, [c_void_p, c_void_p, c_int32, c_void_p]),
