@@ -236,6 +236,18 @@ WM_API int wm_fp8_gemm(const void* aq, const float* as, const void* bq, const fl
                        int32_t m, int32_t n, int32_t k, int32_t a_block_rows, int32_t b_block_rows,
                        int32_t out_is_f32, int32_t accumulate, void* stream);
 
+/* FP8 matrix product  out[m,n] (+)= A[m,k] * B[n,k]^T, stream-ordered: neither synchronises nor allocates, may be
+ * captured.  aq / bq: E4M3 bytes, rows ceil128(k) apart (bytes behind k are not read), 16-byte aligned; as / bs: FP32
+ * scales [ceil(rows / block_rows)][ceil(k / 128)], block rows 1 or 128, any values: each block of 128 along K is
+ * summed in FP32 on the tensor cores and added times the product of its two scales in FP32.
+ * out: rows ld >= n elements apart, BF16 (rounded once) or FP32; accumulate adds into an FP32 out.  k == 0 gives zeros.
+ * wm_fp8_matmul_status synchronises `stream`, reads and clears the device's word: *code = WM_ERR_TIMEOUT when a
+ * bounded wait of an earlier call ran out (that call's out is then incomplete). */
+WM_API int wm_fp8_matmul(const void* aq, const float* as, const void* bq, const float* bs, void* out, int64_t ld,
+                         int32_t m, int32_t n, int32_t k, int32_t a_block_rows, int32_t b_block_rows,
+                         int32_t out_is_f32, int32_t accumulate, void* stream);
+WM_API int wm_fp8_matmul_status(int32_t* code, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * NVFP4 (E2M1 with an E4M3 scale per 16 elements and an FP32 layer scale).
  * wm_nvfp4_quantize: x BF16 [rows][cols] -> data [rows][cols/2] bytes (even element in the low nibble)

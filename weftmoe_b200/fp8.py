@@ -15,10 +15,12 @@ Storage rules:
 """
 from __future__ import annotations
 
+import ctypes
 import weakref
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -174,6 +176,53 @@ def fp8_gemm(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Ten
     return out
 
 
+def _keep(stream, *tensors):
+    """Keeps the storage of operands that were made on another stream until this stream has read them."""
+    for t in tensors:
+        t.record_stream(stream)
+
+
+def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Tensor | None = None,
+               accumulate: bool = False) -> torch.Tensor:
+    """A @ B^T of A [M, K] and B [N, K], blocks of 1 or 128 rows on either side, any scales.
+
+    Enqueues on the current stream and returns; may be captured.  `out` (BF16 or FP32 like `dtype`) may be a
+    slice of a wider tensor: unit column stride, rows at least N apart.  `accumulate` adds into an FP32 `out`."""
+    if not isinstance(a, FP8Tensor) or not isinstance(b, FP8Tensor):
+        raise TypeError("fp8_matmul takes FP8Tensor operands")
+    if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[1] or a.data.device != b.data.device:
+        raise ValueError("FP8 matmul requires [M,K], [N,K] on the same device")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("FP8 matmul output dtype must be BF16 or FP32")
+    if accumulate and (out is None or dtype != torch.float32):
+        raise ValueError("FP8 accumulation requires an existing FP32 output")
+    (m, k), n = a.shape, b.shape[0]
+    device = a.data.device
+    with torch.cuda.device(device):
+        if out is None:
+            out = torch.empty((m, n), dtype=dtype, device=device)
+        else:
+            fits = (isinstance(out, torch.Tensor) and tuple(out.shape) == (m, n) and out.dtype == dtype
+                    and out.device == device and (n <= 1 or out.stride(1) == 1) and (m <= 1 or out.stride(0) >= n))
+            if not fits:
+                raise ValueError("FP8 output shape, dtype, device or layout mismatch")
+        stream = torch.cuda.current_stream()
+        _lib.check(_lib.load().wm_fp8_matmul(
+            _lib.ptr(a.data), _lib.ptr(a.scales), _lib.ptr(b.data), _lib.ptr(b.scales), _lib.ptr(out),
+            out.stride(0) if m > 1 else max(n, 1), m, n, k, a.block_rows, b.block_rows, int(dtype == torch.float32),
+            int(accumulate), stream.cuda_stream))
+        _keep(stream, a.data, a.scales, b.data, b.scales)
+    return out
+
+
+def poll_fp8_matmul() -> None:
+    """Synchronise the current stream and raise if an `fp8_matmul` of this device gave up a wait."""
+    code = ctypes.c_int32()
+    _lib.check(_lib.load().wm_fp8_matmul_status(ctypes.byref(code), torch.cuda.current_stream().cuda_stream))
+    if code.value:
+        raise RuntimeError("fp8_matmul: a device wait ran out; results since the last poll are incomplete")
+
+
 class _ParameterStamp:
     """Identity and in-place version of the parameter tensor a weight was prepared from."""
     __slots__ = ("ref", "version")
@@ -315,3 +364,104 @@ def prepare_fp8_weights(w1, w2, *, training: bool = True, version: int = 0) -> P
         else:
             backward = [None, None]
         return PreparedFP8Weights(a, b, backward[0], backward[1], version, origin, mantissas)
+
+
+class PreparedFP8Linear:
+    """One version of a projection's weight [out, in] in 128 x 128 blocks, and its transpose (the same bytes and
+    scales) for the gradient of the input when prepared for training.  Prepare a new one after each optimizer step."""
+
+    __slots__ = ("weight", "weight_t", "_ready", "_stamps", "_origin", "__weakref__")
+
+    def __init__(self, weight, weight_t, origin):
+        self.weight, self.weight_t, self._origin = weight, weight_t, origin
+        with torch.cuda.device(weight.data.device):
+            self._ready = torch.cuda.Event()
+            self._ready.record()                # preparation kernels were enqueued on this stream
+        self._stamps = self._versions()
+
+    def _versions(self):
+        return tuple(t._version for w in (self.weight, self.weight_t) if w is not None for t in (w.data, w.scales))
+
+    def validate(self, parameter, *, training):
+        if self._versions() != self._stamps:
+            raise RuntimeError("Prepared FP8 weights were modified; prepare a new weight version")
+        if training and self.weight_t is None:
+            raise ValueError("Backward requires weights prepared with training=True")
+        if self._origin is not None:
+            self._origin.check(parameter)
+
+    def wait(self):
+        """Order the current stream after the preparation kernels."""
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().wait_event(self._ready)
+
+
+@torch.inference_mode(False)
+@torch.no_grad()
+def prepare_fp8_linear(weight, *, training: bool = True) -> PreparedFP8Linear:
+    """Quantise a BF16/FP32 weight [out, in] (or import an FP8Tensor with 128 x 128 blocks) for `fp8_linear`."""
+    if isinstance(weight, FP8Tensor):
+        if len(weight.shape) != 2:
+            raise ValueError("Expected a weight [out, in]")
+        straight = _import_quantised(weight)
+        with torch.cuda.device(straight.data.device):
+            flipped = transpose_fp8_weight(straight) if training else None
+            return PreparedFP8Linear(straight, flipped, None)
+    _require_cuda(weight, _SOURCE_DTYPES, "prepare_fp8_linear")
+    if weight.ndim != 2 or 0 in weight.shape:
+        raise ValueError("Expected a weight [out, in]")
+    if training:
+        straight, flipped = _quantize_fp8_weight_pair(weight)
+    else:
+        straight, flipped = quantize_fp8(weight, block_rows=128), None
+    return PreparedFP8Linear(straight, flipped, _ParameterStamp(weight))
+
+
+class _FP8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, prepared):
+        ctx.prepared = prepared
+        ctx.save_for_backward(x, weight)   # the weight: detects optimizer updates before backward
+        return fp8_matmul(quantize_fp8(x), prepared.weight, dtype=x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        prepared = ctx.prepared
+        dx = dweight = None
+        dy = dy.contiguous()
+        if ctx.needs_input_grad[0]:
+            dx = fp8_matmul(quantize_fp8(dy), prepared.weight_t, dtype=x.dtype)
+        if ctx.needs_input_grad[1]:
+            dweight = fp8_matmul(quantize_fp8(dy, transpose=True), quantize_fp8(x, transpose=True),
+                                 dtype=weight.dtype)
+        return dx, dweight, None
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, prepared: PreparedFP8Linear) -> torch.Tensor:
+    """y = x W^T for x [..., in] and W [out, in] on the FP8 tensor cores, the projection beside the FP8 experts.
+
+    x (BF16 or FP32; y has its type) is quantised 1 x 128, the weight comes quantised 128 x 128 from
+    `prepare_fp8_linear(weight)`.  Backward: dx from dy in 1 x 128 blocks and the same weight bytes; dW (of the
+    weight's type) from dy and x in 1 x 128 blocks along the tokens.  Capture a backward pass together with its
+    forward pass."""
+    if not isinstance(prepared, PreparedFP8Linear):
+        raise TypeError("prepared must be PreparedFP8Linear")
+    if not isinstance(x, torch.Tensor) or x.dtype not in _SOURCE_DTYPES or x.ndim < 1:
+        raise ValueError("x must be a BF16 or FP32 tensor [..., in]")
+    if (not isinstance(weight, torch.Tensor) or weight.dtype not in _SOURCE_DTYPES
+            or tuple(weight.shape) != tuple(prepared.weight.shape)):
+        raise ValueError("weight must be the BF16 or FP32 parameter [out, in] that was prepared")
+    if x.shape[-1] != weight.shape[1] or x.device != prepared.weight.data.device or weight.device != x.device:
+        raise ValueError("x, weight and the prepared weight do not match in size or device")
+    training = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+    prepared.validate(weight, training=training and x.requires_grad)
+    rows = x.reshape(-1, x.shape[-1]).contiguous()
+    with torch.cuda.device(x.device):
+        prepared.wait()
+        if training:
+            y = _FP8Linear.apply(rows, weight, prepared)
+        else:
+            y = fp8_matmul(quantize_fp8(rows.detach()), prepared.weight, dtype=x.dtype)
+    return y.view(*x.shape[:-1], weight.shape[0])
