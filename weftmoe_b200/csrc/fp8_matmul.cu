@@ -4,16 +4,20 @@
 //   out[m, n] = sum over K blocks b of  sa[m, b] * sb[n, b] * ( sum over k in b of  a[m, k] * b[n, k] )
 //
 // The inner sum runs on the tensor cores (tcgen05.mma kind::f8f6f4, FP32 accumulator in TMEM, a fresh one for each
-// block of 128); the outer sum runs in FP32 registers of the epilogue warps, which read each block's accumulator
+// block of 128); the outer sum runs in FP32 registers of the adding warps, which read each block's accumulator
 // once and add it times the block's scales.  So any FP32 scales are applied as they are, to operands as they are
 // stored, and the accumulation across blocks is plain FP32.
 //
-// "P" is the operand whose rows lie on the TMEM lanes (128 a tile), "Q" the one whose rows are its columns (BN a tile).
+// "P" is the operand whose rows lie on the TMEM lanes (128 a CTA), "Q" the one whose rows are its columns (BN a tile).
 // P = A, Q = B in general; for few rows of A the roles are swapped (SWAP): the weights' rows fill the lanes and the
 // tokens are BN = 16, 32 or 64 columns, so that no lane is idle and the weights stream through once.
 //
-// Roles of a CTA: warp 0 TMA, warp 1 MMA and TMEM, the others add up the blocks.  S CTAs of a cluster may share one
-// tile, each a range of the blocks; their sums are joined through distributed shared memory in a fixed order.
+// Warps of a CTA: 0 TMA, 1 MMA and TMEM, 2 and 3 fetch the scales, the others add up the blocks.  A stage's `done`
+// barrier, one commit per block, both frees the stage and hands its accumulator to the adding warps.
+// PAIR: two CTAs compute one 256 x 256 tile with cta_group::2, each fetching its own 128 rows of P and half of Q's 256,
+// so a byte of either operand feeds twice the arithmetic of a 128 x 128 tile.
+// Otherwise `split` CTAs of a cluster may share one tile, each a range of the blocks; their sums are joined through
+// distributed shared memory in a fixed order.
 #include "../../include/weftmoe_b200.h"
 #include "gemm.cuh"
 #include "kernels.h"
@@ -30,14 +34,23 @@ struct MatmulArgs {
   const float* p_scales;
   const float* q_scales;
   int p_rows, q_rows;             // M, N or N, M
-  int p_block_rows, q_block_rows; // 1 or 128
+  int p_shift, q_shift;           // log2 of the rows of a scale: 0 or 7
   int kblocks;                    // stride of the scales
   int p_tiles, q_tiles, split;
   void* out;
   long long ld;
-  int out_is_f32, accumulate, vector_store;
+  int out_is_f32, accumulate;
+  int vector_store;               // rows of out are 16-byte aligned
+  int tma_store;                  // ... and tmap_out describes them
 };
 
+// ---------------------------------------------------------------- instructions
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -49,71 +62,130 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16])
 }
 template <int N>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[N]) {
-  static_assert(N == 16 || N == 32, "columns of one load");
-  if constexpr (N == 16) tmem_ld_32x16(taddr, v);
+  static_assert(N == 8 || N == 16 || N == 32, "columns of one load");
+  if constexpr (N == 8) tmem_ld_32x8(taddr, v);
+  else if constexpr (N == 16) tmem_ld_32x16(taddr, v);
   else tmem_ld_32x32(taddr, v);
+}
+// Waits for this thread's TMEM loads.  The registers pass through empty statements behind the wait, so that
+// nothing that reads them is moved before it.
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&v)[N]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+r"(v[j]));
 }
 // 4 bytes global -> shared, or zero.
 __device__ __forceinline__ void copy_async_4(float* dst, const float* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4 : 0)
                : "memory");
 }
-__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-template <int THREADS>
-__device__ __forceinline__ void adders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+// One arrival of this thread on `bar` when its copies so far have landed.
+__device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ float load_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+// Two FP32 multiply-adds in one instruction, on register pairs.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// CTA-pair MMA of 8-bit operands (M = 256: 128 rows in each CTA's TMEM).
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// One commit that arrives on the barrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+// Arrives on an mbarrier of the cluster without a fence over global memory: what the arrival orders are TMEM reads,
+// and those are complete (tcgen05.wait::ld).  With .release.cluster here, once per block, the product of
+// 8192 x 4096 x 4096 took 278 us instead of 171, the difference in the fence.
+__device__ __forceinline__ void arrive_in_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <int REGS>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-// Shared memory of the scales: [2][kScaleChunk][pitch].  Eight lanes copy the eight blocks of one row (one 32-byte
-// sector); the pitch of 4 (mod 32) words keeps those eight and the next three rows in different banks.
-template <int BN, bool Q_COLS>
-struct ScaleTable {
+// ---------------------------------------------------------------- layout
+template <int BN, int EPI, bool SWAP, bool Q_COLS, bool PAIR>
+struct Matmul {
+  static constexpr int kThreads = 128 + 32 * EPI;
+  static constexpr int kCols = BN / (EPI / 4);                   // columns of one adding warp
+  static constexpr int kLoad = kCols / 2 < 32 ? kCols / 2 : 32;  // ... of one TMEM load
+  static constexpr int kRowsP = PAIR ? 256 : 128;                // of a tile
+  static constexpr int kPBytes = 128 * 128;
+  static constexpr int kQBytes = (PAIR ? BN / 2 : BN) * 128;     // this CTA's
+  static constexpr int kStageBytes = kPBytes + kQBytes;
+  static constexpr int kBuffers = BN == 256 ? 2 : 4;             // accumulators in TMEM
+  static constexpr int kColumns = BN * kBuffers < 32 ? 32 : BN * kBuffers;
+  static constexpr int kStages = PAIR ? 4 : BN == 128 ? 5 : 8;
+  static_assert(kStages >= kBuffers, "an adding warp is never a whole round of stages behind the MMA");
+  // Scales: [2][kScaleChunk][pitch] of P, then of Q.  Eight lanes copy the eight blocks of one row (one 32-byte
+  // sector); the pitch of 4 (mod 32) words keeps those eight and the next three rows in different banks.
   static constexpr int kPitchP = 128 + 4;
   static constexpr int kPitchQ = Q_COLS ? BN + 4 : 4;
-  static constexpr int kWords = 2 * kScaleChunk * (kPitchP + kPitchQ);
+  static constexpr int kScaleBytes = 2 * kScaleChunk * (kPitchP + kPitchQ) * 4;
+  static constexpr int kStoreBytes = SWAP ? 0 : kCols * 32 * 2;  // staging of one adding warp
+  static constexpr int kScalesAt = kStages * kStageBytes + EPI * kStoreBytes;
+  static constexpr int kBarriersAt = kScalesAt + kScaleBytes;
+  static constexpr int kTotal = kBarriersAt + 256 + 1024;
+  static_assert(kScalesAt % 16 == 0 && kTotal <= 227 * 1024, "shared memory");
+  static_assert(PAIR || BN * 128 * 4 <= kStages * kStageBytes, "the joined sums fit in the stages");
+  // PAIR: the four service warps give registers to the eight adding warps: 128 x 56 + 256 x 224 = 384 x 168, what
+  // the block is launched with (checked before the first launch).
+  static constexpr int kRegisters = 168, kLow = 56, kHigh = 224;
+  static_assert(!PAIR || 128 * kLow + 256 * kHigh <= kThreads * kRegisters, "registers of the block");
 };
 
-template <int BN, int EPI, bool Q_COLS>
-__device__ __forceinline__ void fetch_scales(const MatmulArgs& a, float* table, int buffer, int p0, int q0, int kb0,
-                                             int kb1, int thread) {
-  using T = ScaleTable<BN, Q_COLS>;
-  float* tp = table + buffer * kScaleChunk * T::kPitchP;
-  float* tq = table + 2 * kScaleChunk * T::kPitchP + buffer * kScaleChunk * T::kPitchQ;
-  const int kb = thread & 7;
-  const bool in = kb0 + kb < kb1;
-  for (int r = thread >> 3; r < 128; r += EPI * 4) {
-    const bool there = in && p0 + r < a.p_rows;
-    const float* src = a.p_scales + (there ? static_cast<long long>((p0 + r) / a.p_block_rows) * a.kblocks + kb0 + kb : 0);
-    copy_async_4(tp + kb * T::kPitchP + r, src, there);
-  }
-  constexpr int kEntries = Q_COLS ? BN : BN / 128;
-  for (int c = thread >> 3; c < kEntries; c += EPI * 4) {
-    const int row = q0 + (Q_COLS ? c : c * 128);
-    const bool there = in && row < a.q_rows;
-    const float* src = a.q_scales + (there ? static_cast<long long>(row / a.q_block_rows) * a.kblocks + kb0 + kb : 0);
-    copy_async_4(tq + kb * T::kPitchQ + c, src, there);
-  }
-  copy_async_commit();
+struct Tile {
+  int p0, q0;   // first rows of this CTA's P, of the tile's Q
+};
+// Tiles are walked in groups of eight rows of tiles, so that the CTAs in flight share both operands in L2.
+template <int ROWS_P, int BN>
+__device__ __forceinline__ Tile tile_at(const MatmulArgs& a, int tile) {
+  const int per_group = 8 * a.q_tiles;
+  const int group = tile / per_group, rem = tile - group * per_group;
+  const int rows = min(8, a.p_tiles - group * 8);
+  return Tile{(group * 8 + rem % rows) * ROWS_P, rem / rows * BN};
 }
 
-template <int BN, int EPI, bool Q_COLS>
-struct MatmulSmem {
-  static constexpr int kPBytes = 128 * 128;
-  static constexpr int kQBytes = BN * 128;
-  static constexpr int kStageBytes = kPBytes + kQBytes;
-  static constexpr int kBuffers = BN == 256 ? 2 : 4;       // accumulators in TMEM
-  static constexpr int kColumns = BN * kBuffers < 32 ? 32 : BN * kBuffers;
-  static constexpr int kStages = BN >= 128 ? 5 : 8;
-  static constexpr int kScaleBytes = ScaleTable<BN, Q_COLS>::kWords * 4;
-  static constexpr int kTotal = kStages * kStageBytes + kScaleBytes + 256 + 1024;
-  static_assert(BN * 128 * 4 <= kStages * kStageBytes, "the joined sums fit in the stages");
-};
-
-// One column of a finished tile.
+// ---------------------------------------------------------------- results
 template <bool SWAP>
 __device__ __forceinline__ void store_one(const MatmulArgs& a, int p, int q, float v) {
   const long long at = SWAP ? static_cast<long long>(q) * a.ld + p : static_cast<long long>(p) * a.ld + q;
@@ -152,35 +224,82 @@ __device__ __forceinline__ void store_row(const MatmulArgs& a, int p, int q, con
   for (int j = 0; j < COLS; ++j)
     if (q + j < a.q_rows) store_one<false>(a, p, q + j, v[j]);
 }
+// A warp's 32 rows x 2 * PAIRS columns through shared memory and TMA: boxes of 32 rows x 128 bytes, 16-byte pieces
+// swizzled by the row as the map says.  The tensor map clips what lies outside the matrix.
+template <int PAIRS>
+__device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorMap* tmap, uint8_t* staging, int p, int q,
+                                            int lane, const uint64_t (&sum)[PAIRS]) {
+  constexpr int kBoxes = PAIRS / 32;                     // boxes that fit in the staging at once
+  const int passes = a.out_is_f32 ? 2 : 1;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == passes) break;
+    if (lane == 0) bulk_wait_group_read<0>();            // the boxes before these have left the staging
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b) {
+      uint8_t* line = staging + b * 4096 + lane * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 w;
+        if (a.out_is_f32) {
+          const int from = ((pass * kBoxes + b) * 32 + c * 4) / 2;
+          const float2 x = halves_of(sum[from]), y = halves_of(sum[from + 1]);
+          w = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
+        } else {
+          const int from = (b * 64 + c * 8) / 2;
+          const float2 x = halves_of(sum[from]), y = halves_of(sum[from + 1]), z = halves_of(sum[from + 2]),
+                       t = halves_of(sum[from + 3]);
+          w = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(y.x, y.y), pack_bf16x2(z.x, z.y), pack_bf16x2(t.x, t.y));
+        }
+        *reinterpret_cast<uint4*>(line + ((c ^ (lane & 7)) << 4)) = w;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+#pragma unroll
+      for (int b = 0; b < kBoxes; ++b) {
+        const int x = q + (a.out_is_f32 ? (pass * kBoxes + b) * 32 : b * 64);
+        if (p < a.p_rows && x < a.q_rows) tma_store_2d(tmap, staging + b * 4096, x, p);
+      }
+      bulk_commit_group();
+    }
+  }
+}
 
-template <int BN, int EPI, bool SWAP, bool Q_COLS>
-__global__ void __launch_bounds__(64 + 32 * EPI, 1)
+// ---------------------------------------------------------------- the kernel
+template <int BN, int EPI, bool SWAP, bool Q_COLS, bool PAIR>
+__global__ void __launch_bounds__(128 + 32 * EPI, 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
-                  const MatmulArgs a) {
-  using S = MatmulSmem<BN, EPI, Q_COLS>;
-  using T = ScaleTable<BN, Q_COLS>;
-  constexpr int kCols = BN / (EPI / 4);                   // columns of one adding warp
-  constexpr int kLoad = kCols < 32 ? kCols : 32;
+                  const __grid_constant__ CUtensorMap tmap_out, const MatmulArgs a) {
+  using S = Matmul<BN, EPI, SWAP, Q_COLS, PAIR>;
+  constexpr int kCols = S::kCols, kLoad = S::kLoad;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* scales = reinterpret_cast<float*>(smem + S::kStages * S::kStageBytes);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStageBytes + S::kScaleBytes);
-  uint64_t* empty_bar = full_bar + S::kStages;
-  uint64_t* tmem_full = empty_bar + S::kStages;
-  uint64_t* tmem_empty = tmem_full + S::kBuffers;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tmem_empty + S::kBuffers);
+  float* scales_p = reinterpret_cast<float*>(smem + S::kScalesAt);
+  float* scales_q = scales_p + 2 * kScaleChunk * S::kPitchP;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kBarriersAt);   // PAIR: the leader's is used
+  uint64_t* done_bar = full_bar + S::kStages;                                // in both CTAs
+  uint64_t* tmem_empty = done_bar + S::kStages;                              // the leader's
+  uint64_t* scale_full = tmem_empty + S::kBuffers;
+  uint64_t* scale_empty = scale_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(scale_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = PAIR ? static_cast<int>(cluster_ctarank()) : 0;            // 0 = leader
+  const int part = !PAIR && a.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(full_bar + s, 1);
-      mbar_init(empty_bar + s, 1);
+      mbar_init(done_bar + s, 1);
     }
-    for (int s = 0; s < S::kBuffers; ++s) {
-      mbar_init(tmem_full + s, 1);
-      mbar_init(tmem_empty + s, EPI);
+    for (int s = 0; s < S::kBuffers; ++s) mbar_init(tmem_empty + s, PAIR ? 2 * EPI : EPI);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(scale_full + s, 64);
+      mbar_init(scale_empty + s, EPI);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -193,36 +312,45 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  const int part = a.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int group = PAIR ? 2 : a.split;    // CTAs of a tile
   const int kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * part / a.split);
   const int kb1 = static_cast<int>(static_cast<long long>(a.kblocks) * (part + 1) / a.split);
   const int tiles = a.p_tiles * a.q_tiles;
-  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
+  const int first = blockIdx.x / group, step = gridDim.x / group;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    if constexpr (PAIR) registers_down<S::kLow>();
+    if (warp == 0 && lane == 0) {
+      // ------------------------------------------------------------ TMA
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first; ok && tile < tiles; tile += step) {
-        const int p0 = tile % a.p_tiles * 128, q0 = tile / a.p_tiles * BN;
+        const Tile t = tile_at<S::kRowsP, BN>(a, tile);
         for (int kb = kb0; kb < kb1; ++kb) {
-          ok = mbar_wait(empty_bar + stage, phase ^ 1, abort_flag, &g_matmul_status, kStatusTimeoutSmemEmpty);
+          ok = mbar_wait(done_bar + stage, phase ^ 1, abort_flag, &g_matmul_status, kStatusTimeoutSmemEmpty);
           if (!ok) break;
           uint8_t* sp = smem + stage * S::kStageBytes;
-          mbar_expect_tx(full_bar + stage, S::kStageBytes);
-          tma_load_2d(sp, &tmap_p, full_bar + stage, kb * 128, p0);
-          tma_load_2d(sp + S::kPBytes, &tmap_q, full_bar + stage, kb * 128, q0);
+          if constexpr (PAIR) {
+            const uint32_t bar = map_to_cta(smem_u32(full_bar + stage), 0);
+            if (cta == 0) mbar_expect_tx(full_bar + stage, 2 * S::kStageBytes);
+            tma_load_2d_pair(sp, &tmap_p, bar, kb * 128, t.p0 + cta * 128);
+            tma_load_2d_pair(sp + S::kPBytes, &tmap_q, bar, kb * 128, t.q0 + cta * (BN / 2));
+          } else {
+            mbar_expect_tx(full_bar + stage, S::kStageBytes);
+            tma_load_2d(sp, &tmap_p, full_bar + stage, kb * 128, t.p0);
+            tma_load_2d(sp + S::kPBytes, &tmap_q, full_bar + stage, kb * 128, t.q0);
+          }
           if (++stage == S::kStages) { stage = 0; phase ^= 1; }
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc(0u, 128, BN, 0u, 0u);
+    } else if (warp == 1 && lane == 0 && cta == 0) {
+      // ------------------------------------------------------------ MMA
+      constexpr uint32_t idesc = umma_idesc(0u, S::kRowsP, BN, 0u, 0u);
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
@@ -235,95 +363,170 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
           const uint32_t sp = smem_u32(smem + stage * S::kStageBytes);
           const uint64_t dp = umma_desc_sw128(sp, 0, 1024), dq = umma_desc_sw128(sp + S::kPBytes, 0, 1024);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
-          umma_commit(empty_bar + stage);
-          umma_commit(tmem_full + buffer);
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (PAIR) umma_f8_pair(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
+            else umma_f8(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
+          }
+          if constexpr (PAIR) umma_commit_both(done_bar + stage);
+          else umma_commit(done_bar + stage);
           if (++stage == S::kStages) { stage = 0; phase ^= 1; }
           if (++buffer == S::kBuffers) { buffer = 0; buffer_phase ^= 1; }
         }
       }
+    } else if (warp >= 2) {
+      // ------------------------------------------------------------ scales
+      const int kb = lane & 7, row = (threadIdx.x - 64) >> 3;
+      int held = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < tiles; tile += step) {
+        const Tile t = tile_at<S::kRowsP, BN>(a, tile);
+        const int p0 = t.p0 + cta * 128;
+        for (int chunk = kb0; chunk < kb1; chunk += kScaleChunk) {
+          ok = mbar_wait(scale_empty + held, phase ^ 1, abort_flag, &g_matmul_status, kStatusTimeoutSmemEmpty);
+          if (!ok) break;
+          float* to = scales_p + (held * kScaleChunk + kb) * S::kPitchP;
+          const bool in = chunk + kb < kb1;
+#pragma unroll 4
+          for (int r = row; r < 128; r += 8) {
+            const bool there = in && p0 + r < a.p_rows;
+            copy_async_4(to + r, a.p_scales + (there ? static_cast<long long>((p0 + r) >> a.p_shift) * a.kblocks + chunk + kb : 0),
+                         there);
+          }
+          to = scales_q + (held * kScaleChunk + kb) * S::kPitchQ;
+          constexpr int kEntries = Q_COLS ? BN : BN / 128;
+#pragma unroll 4
+          for (int c = row; c < kEntries; c += 8) {
+            const int r = t.q0 + (Q_COLS ? c : c * 128);
+            const bool there = in && r < a.q_rows;
+            copy_async_4(to + c, a.q_scales + (there ? static_cast<long long>(r >> a.q_shift) * a.kblocks + chunk + kb : 0),
+                         there);
+          }
+          copy_async_arrive(scale_full + held);
+          if (++held == 2) { held = 0; phase ^= 1; }
+        }
+      }
+      copy_async_wait();
     }
   } else {
-    const int thread = threadIdx.x - 64;
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const int row = q * 32 + lane, col0 = half * kCols;
-    int buffer = 0, held = 0;
-    uint32_t buffer_phase = 0;
-    bool ok = true;   // a wait that runs out skips the arithmetic; the barriers below are still met by every warp
-    if (first < tiles)
-      fetch_scales<BN, EPI, Q_COLS>(a, scales, 0, first % a.p_tiles * 128, first / a.p_tiles * BN, kb0, kb1, thread);
-    for (int tile = first; tile < tiles; tile += step) {
-      const int p0 = tile % a.p_tiles * 128, q0 = tile / a.p_tiles * BN;
-      float sum[kCols];
+    // ------------------------------------------------------------ sums
+    if constexpr (PAIR) registers_up<S::kHigh>();
+    const int q = warp & 3, col0 = ((warp - 4) >> 2) * kCols;
+    const int row = q * 32 + lane;
+    const uint32_t from = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + col0;
+    int stage = 0, buffer = 0, held = 0;
+    uint32_t phase = 0, held_phase = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += step) {
+      const Tile t = tile_at<S::kRowsP, BN>(a, tile);
+      const int p0 = t.p0 + cta * 128;
+      uint64_t sum[kCols / 2];
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
-      for (int chunk = kb0; chunk < kb1; chunk += kScaleChunk) {
-        copy_async_wait();
-        adders_sync<EPI * 32>();   // this chunk is here, and the other buffer is no longer read
-        if (chunk + kScaleChunk < kb1)
-          fetch_scales<BN, EPI, Q_COLS>(a, scales, held ^ 1, p0, q0, chunk + kScaleChunk, kb1, thread);
-        else if (tile + step < tiles)
-          fetch_scales<BN, EPI, Q_COLS>(a, scales, held ^ 1, (tile + step) % a.p_tiles * 128,
-                                        (tile + step) / a.p_tiles * BN, kb0, kb1, thread);
-        const float* tp = scales + held * kScaleChunk * T::kPitchP + row;
-        const float* tq = scales + 2 * kScaleChunk * T::kPitchP + held * kScaleChunk * T::kPitchQ;
-        const int last = min(kScaleChunk, kb1 - chunk);
-        for (int kb = 0; kb < last; ++kb) {
-          ok = ok && mbar_wait(tmem_full + buffer, buffer_phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
-          if (!ok) continue;
-          tc_fence_after();
-          float factor = tp[kb * T::kPitchP];
-          if constexpr (!Q_COLS) factor *= tq[kb * T::kPitchQ + col0 / 128];
+      for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
+      // Loads run ahead of the additions by kLoad columns, across blocks too.
+      uint32_t v[2][kLoad];
+      ok = mbar_wait(done_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld_cols<kLoad>(from + buffer * BN, v[0]);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int in_chunk = (kb - kb0) & (kScaleChunk - 1);
+        if (in_chunk == 0) {
+          ok = mbar_wait(scale_full + held, held_phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
+          if (!ok) break;
+        }
+        const float* tq = scales_q + (held * kScaleChunk + in_chunk) * S::kPitchQ + (Q_COLS ? col0 : col0 / 128);
+        float factor = scales_p[(held * kScaleChunk + in_chunk) * S::kPitchP + row];
+        if constexpr (!Q_COLS) factor *= *tq;
+        const uint64_t factors = pair_of(factor, factor);
 #pragma unroll
-          for (int c = 0; c < kCols / kLoad; ++c) {
-            uint32_t v[kLoad];
-            tmem_ld_cols<kLoad>(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buffer * BN + col0 + c * kLoad, v);
-            tmem_ld_wait();
-            if (c == kCols / kLoad - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(tmem_empty + buffer);
+        for (int c = 0; c < kCols / kLoad; ++c) {
+          tmem_ld_wait_for<kLoad>(v[c & 1]);
+          if (c + 1 < kCols / kLoad) {
+            tmem_ld_cols<kLoad>(from + buffer * BN + (c + 1) * kLoad, v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR) arrive_in_cluster(map_to_cta(smem_u32(tmem_empty + buffer), 0));
+              else mbar_arrive(tmem_empty + buffer);
             }
-#pragma unroll
-            for (int j = 0; j < kLoad; ++j) {
-              float f = factor;
-              if constexpr (Q_COLS) f *= tq[kb * T::kPitchQ + col0 + c * kLoad + j];
-              sum[c * kLoad + j] = fmaf(f, __uint_as_float(v[j]), sum[c * kLoad + j]);
+            if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+            if (++buffer == S::kBuffers) buffer = 0;
+            if (kb + 1 < kb1) {
+              ok = mbar_wait(done_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
+              tc_fence_after();
+              tmem_ld_cols<kLoad>(from + buffer * BN, v[(c + 1) & 1]);
             }
           }
-          if (++buffer == S::kBuffers) { buffer = 0; buffer_phase ^= 1; }
+#pragma unroll
+          for (int j = 0; j < kLoad / 2; ++j) {
+            const uint64_t x = pair_of(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
+            uint64_t f = factors;
+            if constexpr (Q_COLS) {
+              const float2 w = *reinterpret_cast<const float2*>(tq + c * kLoad + 2 * j);
+              f = mul_pair(f, pair_of(w.x, w.y));
+            }
+            sum[c * (kLoad / 2) + j] = fma_pair(f, x, sum[c * (kLoad / 2) + j]);
+          }
         }
-        held ^= 1;
+        if (in_chunk == kScaleChunk - 1 || kb + 1 == kb1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(scale_empty + held);
+          if (++held == 2) { held = 0; held_phase ^= 1; }
+        }
+        if (!ok) break;
       }
-      if (a.split > 1) {   // one tile per CTA: the stages are no longer written
+      tmem_ld_wait();
+      if (!ok) break;
+      if (!PAIR && a.split > 1) {   // one tile per CTA: its stages are read and no longer written
         float* mine = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) mine[(col0 + j) * 128 + row] = sum[j];
-      } else if (ok && p0 + row < a.p_rows) {
-        if constexpr (SWAP) {
+        for (int j = 0; j < kCols / 2; ++j) {
+          const float2 w = halves_of(sum[j]);
+          mine[(col0 + 2 * j) * 128 + row] = w.x;
+          mine[(col0 + 2 * j + 1) * 128 + row] = w.y;
+        }
+      } else if constexpr (SWAP) {
 #pragma unroll
-          for (int j = 0; j < kCols; ++j)
-            if (q0 + col0 + j < a.q_rows) store_one<true>(a, p0 + row, q0 + col0 + j, sum[j]);
-        } else {
-          store_row<kCols>(a, p0 + row, q0 + col0, sum);
+        for (int j = 0; j < kCols / 2; ++j) {
+          const float2 w = halves_of(sum[j]);
+          if (p0 + row < a.p_rows && t.q0 + col0 + 2 * j < a.q_rows) store_one<true>(a, p0 + row, t.q0 + col0 + 2 * j, w.x);
+          if (p0 + row < a.p_rows && t.q0 + col0 + 2 * j + 1 < a.q_rows)
+            store_one<true>(a, p0 + row, t.q0 + col0 + 2 * j + 1, w.y);
+        }
+      } else if (a.tma_store) {
+        store_boxes<kCols / 2>(a, &tmap_out, smem + S::kStages * S::kStageBytes + (warp - 4) * S::kStoreBytes,
+                               p0 + q * 32, t.q0 + col0, lane, sum);
+      } else if (p0 + row < a.p_rows) {
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
+          float w[32];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 h = halves_of(sum[c * 16 + j]);
+            w[2 * j] = h.x;
+            w[2 * j + 1] = h.y;
+          }
+          store_row<32>(a, p0 + row, t.q0 + col0 + c * 32, w);
         }
       }
     }
+    if (!SWAP && lane == 0) bulk_wait_group_read<0>();   // the staging stays until it is read
   }
-  if (a.split > 1) {
-    __syncwarp();
+  __syncwarp();
+  if (!PAIR && a.split > 1) {
     cluster_sync_all();
-    if (warp >= 2 && first < tiles && !*abort_flag) {
-      const int p0 = first % a.p_tiles * 128, q0 = first / a.p_tiles * BN;
+    if (warp >= 4 && first < tiles && !*abort_flag) {
+      const Tile t = tile_at<S::kRowsP, BN>(a, first);
       const int row = (warp & 3) * 32 + lane;
       const int cols = BN / a.split;                                        // this CTA's columns of the tile
       const uint32_t base = smem_u32(smem);
-      for (int c = (warp - 2) >> 2; c < cols; c += EPI / 4) {
+      for (int c = (warp - 4) >> 2; c < cols; c += EPI / 4) {
         const int col = part * cols + c;
         float v = 0.0f;
         for (int s = 0; s < a.split; ++s) v += load_cluster(map_to_cta(base + (col * 128 + row) * 4, s));
-        if (p0 + row < a.p_rows && q0 + col < a.q_rows) store_one<SWAP>(a, p0 + row, q0 + col, v);
+        if (t.p0 + row < a.p_rows && t.q0 + col < a.q_rows) store_one<SWAP>(a, t.p0 + row, t.q0 + col, v);
       }
     }
     __syncwarp();
@@ -331,37 +534,58 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // the peer's shared memory and barriers stay valid until both are done
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, S::kColumns);
   }
 }
 
-template <int BN, int EPI, bool SWAP, bool Q_COLS>
-int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, MatmulArgs a, int sms, cudaStream_t stream) {
-  auto kernel = fp8_matmul_kernel<BN, EPI, SWAP, Q_COLS>;
-  constexpr int smem = MatmulSmem<BN, EPI, Q_COLS>::kTotal;
+template <int BN, int EPI, bool SWAP, bool Q_COLS, bool PAIR>
+int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tout, MatmulArgs a, int sms,
+                  cudaStream_t stream) {
+  using S = Matmul<BN, EPI, SWAP, Q_COLS, PAIR>;
+  auto kernel = fp8_matmul_kernel<BN, EPI, SWAP, Q_COLS, PAIR>;
   static PerDeviceOnce configured;  // one table per template instantiation
-  if (int rc = opt_in_dynamic_smem(kernel, smem, configured)) return rc;
-  a.p_tiles = (a.p_rows + 127) / 128;
+  if (int rc = opt_in_dynamic_smem(kernel, S::kTotal, configured)) return rc;
+  if constexpr (PAIR) {
+    static int registers = 0;   // what the kernel was built with
+    if (registers == 0) {
+      cudaFuncAttributes attributes{};
+      WM_CUDA(cudaFuncGetAttributes(&attributes, kernel));
+      registers = attributes.numRegs;
+    }
+    if (registers != S::kRegisters) {
+      set_error("wm_fp8_matmul: the kernel was built with %d registers, its warps share out %d", registers, S::kRegisters);
+      return WM_ERR_STATE;
+    }
+  }
+  a.p_tiles = (a.p_rows + S::kRowsP - 1) / S::kRowsP;
   a.q_tiles = (a.q_rows + BN - 1) / BN;
   const long long tiles = static_cast<long long>(a.p_tiles) * a.q_tiles;
+  if (tiles > 0x3fffffff) {
+    set_error("wm_fp8_matmul: more than 2^30 tiles");
+    return WM_ERR_INVALID;
+  }
   // Few tiles: 2, 4 or 8 CTAs take a share of the blocks each, while every SM still gets at most one CTA
   // and every CTA two blocks.
   a.split = 1;
-  while (a.split < 8 && tiles * a.split * 2 <= sms && a.kblocks / (a.split * 2) >= 2) a.split *= 2;
+  if (!PAIR)
+    while (a.split < 8 && tiles * a.split * 2 <= sms && a.kblocks / (a.split * 2) >= 2) a.split *= 2;
+  const int group = PAIR ? 2 : a.split;
+  const long long groups = tiles * group <= sms ? tiles : sms / group;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : tiles < sms ? tiles : sms));
-  config.blockDim = dim3(64 + 32 * EPI);
-  config.dynamicSmemBytes = smem;
+  config.gridDim = dim3(static_cast<unsigned>(groups * group));
+  config.blockDim = dim3(S::kThreads);
+  config.dynamicSmemBytes = S::kTotal;
   config.stream = stream;
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = a.split;
+  cluster.val.clusterDim.x = group;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  WM_CUDA(cudaLaunchKernelEx(&config, kernel, tp, tq, a));
+  WM_CUDA(cudaLaunchKernelEx(&config, kernel, tp, tq, tout, a));
   count_launch();
   return WM_OK;
 }
@@ -399,16 +623,18 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   int sms = 0, dev = 0;
   WM_CUDA(cudaGetDevice(&dev));
   WM_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  // Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.
+  // Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  Pairs of SMs take 256 x 256 tiles
+  // where those alone fill half of the pairs.
   const bool swap = m <= 64;
+  const bool pairs = !swap && static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * 4 >= sms;
   const int bn = swap ? (m <= 16 ? 16 : m <= 32 ? 32 : 64) : 128;
   MatmulArgs a{};
   a.p_scales = swap ? bs : as;
   a.q_scales = swap ? as : bs;
   a.p_rows = swap ? n : m;
   a.q_rows = swap ? m : n;
-  a.p_block_rows = swap ? b_block_rows : a_block_rows;
-  a.q_block_rows = swap ? a_block_rows : b_block_rows;
+  a.p_shift = (swap ? b_block_rows : a_block_rows) == 128 ? 7 : 0;
+  a.q_shift = (swap ? a_block_rows : b_block_rows) == 128 ? 7 : 0;
   a.kblocks = kblocks;
   a.out = out;
   a.ld = ld;
@@ -419,13 +645,19 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   CUtensorMap tp, tq;
   if (int rc = make_tmap_2d(&tp, swap ? bq : aq, 1, k, a.p_rows, pitch, 128, 128)) return rc;
   if (int rc = make_tmap_2d(&tq, swap ? aq : bq, 1, k, a.q_rows, pitch, 128, bn)) return rc;
-  if (swap) {
-    if (bn == 16) return launch_matmul<16, 4, true, true>(tp, tq, a, sms, stream);
-    if (bn == 32) return launch_matmul<32, 4, true, true>(tp, tq, a, sms, stream);
-    return launch_matmul<64, 4, true, true>(tp, tq, a, sms, stream);
-  }
-  return a.q_block_rows == 128 ? launch_matmul<128, 8, false, false>(tp, tq, a, sms, stream)
-                               : launch_matmul<128, 8, false, true>(tp, tq, a, sms, stream);
+  CUtensorMap tout = tp;   // not read without tma_store
+  a.tma_store = !swap && a.vector_store && !accumulate;
+  if (a.tma_store)
+    if (int rc = make_tmap_2d(&tout, out, element, n, m, static_cast<uint64_t>(ld) * element, 128 / element, 32)) return rc;
+  const bool by_column = a.q_shift == 0;
+  if (bn == 16) return launch_matmul<16, 4, true, true, false>(tp, tq, tout, a, sms, stream);
+  if (bn == 32) return launch_matmul<32, 4, true, true, false>(tp, tq, tout, a, sms, stream);
+  if (bn == 64) return launch_matmul<64, 4, true, true, false>(tp, tq, tout, a, sms, stream);
+  if (pairs)
+    return by_column ? launch_matmul<256, 8, false, true, true>(tp, tq, tout, a, sms, stream)
+                     : launch_matmul<256, 8, false, false, true>(tp, tq, tout, a, sms, stream);
+  return by_column ? launch_matmul<128, 8, false, true, false>(tp, tq, tout, a, sms, stream)
+                   : launch_matmul<128, 8, false, false, false>(tp, tq, tout, a, sms, stream);
 }
 
 extern "C" int wm_fp8_matmul_status(int32_t* code, void* stream_) {
