@@ -13,15 +13,18 @@
 // second kernel, so results do not depend on the order in which blocks run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "../../include/weftmoe_b200.h"
 #include "kernels.h"
+#include "ptx.cuh"
 
 using namespace wm;
 
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kFinishWarps = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxBlocks = 1184;  // 148 SMs x 8
 constexpr unsigned kAll = 0xffffffffu;
@@ -29,23 +32,14 @@ constexpr unsigned kAll = 0xffffffffu;
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }  // the gradient's type
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }             // is the logits'
+__device__ __forceinline__ void put(float& p, float v) { p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16& p, float v) { p = __float2bfloat16_rn(v); }  // the gradient's type
+__device__ __forceinline__ void put(__half& p, float v) { p = __float2half_rn(v); }             // is the logits'
 
-__device__ __forceinline__ float warp_sum(float v) {
+template <class F>
+__device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
-  return v;
-}
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
-  return v;
-}
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
   return v;
 }
 // Unsigned words in the order of the floats; 0 is below every one of them and means "not available".
@@ -61,6 +55,34 @@ __device__ __forceinline__ unsigned long long ordered(double v) {
   v += 0.0;
   const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(v));
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+// The largest of the lanes' values, which holds no NaN.
+__device__ __forceinline__ float warp_max(float v) { return unordered(__reduce_max_sync(kAll, ordered(v))); }
+// The larger one; NaN if either is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 1 / y to one unit in the last place, for normal y below 2^126.
+__device__ __forceinline__ float reciprocal(float y) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return r;
+}
+// 2^t by the exponent unit, two units in the last place; 0 at -inf.
+__device__ __forceinline__ float power_of_2(float t) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+// Exponentials are powers of 2 of x log2 e.  exp(x - top) is 2^(x log2 e - c) with c the rounded top log2 e: the
+// rounding of c is a factor that all terms of a row share and that their shares do not see, the fused product rounds
+// like the subtraction of the definition.
+constexpr float kLog2E = 1.44269504f;
+constexpr float kHuge = 1e30f;   // beyond it top log2 e may overflow, and differences are 0 or vast
+__device__ __forceinline__ float exp_below(float x, float top) {
+  return power_of_2(fabsf(top) < kHuge ? fmaf(x, kLog2E, -top * kLog2E) : (x - top) * kLog2E);
 }
 
 struct Rows {
@@ -94,137 +116,293 @@ __device__ __forceinline__ bool row_live(const Rows& a, int row, int b) {
   return a.sequences == nullptr || (b < a.num_sequences && row >= __ldg(a.sequences));
 }
 
-template <class T, int V>
-__device__ __forceinline__ void load_row(const Rows& a, int row, int lane, float (&x)[V]) {
-  const T* p = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.stride;
+// Which experts a lane holds: pieces of VEC neighbours, so that a row moves in accesses of VEC elements.
+// Experts rise with the slot, which is what the order of ties relies on.
+template <int VEC>
+__device__ __forceinline__ int expert_of(int slot, int lane) {
+  return slot / VEC * (32 * VEC) + lane * VEC + slot % VEC;
+}
+template <class T, int VEC>
+struct alignas(sizeof(T) * VEC) Piece {
+  T v[VEC];
+};
+template <class T, int V, int VEC>
+__device__ __forceinline__ void load_row(const Rows& a, long long row, int lane, float (&x)[V]) {
+  const T* p = static_cast<const T*>(a.logits) + row * a.stride;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int e = j * 32 + lane;
-    x[j] = e < a.experts ? as_float(p[e]) : -INFINITY;
+  for (int j = 0; j < V; j += VEC) {
+    const int e = expert_of<VEC>(j, lane);
+    if (e < a.experts) {   // experts % VEC == 0: a piece is whole or absent
+      const Piece<T, VEC> w = *reinterpret_cast<const Piece<T, VEC>*>(p + e);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[j + i] = as_float(w.v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[j + i] = -INFINITY;
+    }
+  }
+}
+template <class T, int V, int VEC>
+__device__ __forceinline__ void store_row(T* out, int experts, int lane, const float (&d)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; j += VEC) {
+    const int e = expert_of<VEC>(j, lane);
+    if (e < experts) {
+      Piece<T, VEC> w;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) put(w.v[i], d[j + i]);
+      *reinterpret_cast<Piece<T, VEC>*>(out + e) = w;
+    }
   }
 }
 
-// What a row's arithmetic needs of the whole row.  top: the largest logit.  For softmax s_e = exp(x_e - top) / sum;
-// for sigmoid, p_e = hat(x_e) / sum with hat(x) = s(x) * exp(-min(top, 0)): a row of very negative logits keeps
-// its shares.
-struct RowStats {
-  float top, sum;
-  bool bad, any;  // bad: NaN (or, for softmax, +inf) among the logits; any: an available expert
-};
-__device__ __forceinline__ float sigmoid_hat(float x, float top) {
+// s = 1 / (1 + E) with E = exp(-x), and its complement E s, neither of which cancels.  Below x = -87, where s is no
+// normal number, both are 0.
+__device__ __forceinline__ float sigmoid_of(float x, float& rest) {
+  const float e = power_of_2(fminf(-x * kLog2E, 127.5f));
+  const float s = reciprocal(1.0f + e);
+  rest = e * s;
+  return s;
+}
+// s(x) * exp(-min(top, 0)), for shares of a row whose largest logit `top` is so low that its sigmoids vanish.
+__device__ __forceinline__ float sigmoid_far(float x, float top) {
   return expf(fminf(x, 0.0f) - fminf(top, 0.0f)) / (1.0f + expf(-fabsf(x)));
 }
-// 1 - s(x) without cancellation.
-__device__ __forceinline__ float sigmoid_rest(float x) { return 1.0f / (1.0f + expf(x)); }
+constexpr float kFar = -60.0f;   // sigmoids of a row with a logit above this are normal numbers
 
-// h[j]: exp(x - top) or hat(x); the share of the row is h / sum.
+// Of a row: its largest logit, whether an expert is available, and whether it has no distribution (NaN, or for
+// softmax +inf, among its logits).
+struct RowTop {
+  float top;
+  bool bad, any;
+};
 template <int V>
-__device__ __forceinline__ RowStats row_stats(const float (&x)[V], bool sigmoid, float (&h)[V]) {
-  RowStats r;
-  float top = -INFINITY;
-  bool bad = false;
+__device__ __forceinline__ RowTop row_top(const float (&x)[V], bool sigmoid) {
+  RowTop r;
+  float top = x[0];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    top = fmaxf(top, x[j]);
-    bad |= x[j] != x[j] || (!sigmoid && x[j] == INFINITY);
-  }
-  r.top = warp_max(top);
-  r.bad = __any_sync(kAll, bad);
+  for (int j = 1; j < V; ++j) top = max_or_nan(top, x[j]);
+  r.bad = __any_sync(kAll, top != top);
+  r.top = r.bad ? 0.0f : warp_max(top);
+  r.bad |= !sigmoid && r.top == INFINITY;
   r.any = r.top > -INFINITY;
-  float sum = 0.0f;
-  if (r.any) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      h[j] = sigmoid ? sigmoid_hat(x[j], r.top) : expf(x[j] - r.top);
-      sum += h[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = 0.0f;
-  }
-  r.sum = warp_sum(sum);
   return r;
 }
-
-// K rounds of a warp-wide maximum.  Lane k gets choice k: its expert (-1 when none is left) and its logit.
+// h[j] such that h / sum is the row's share: exp(x - top), or the sigmoid (with its complement in rest).
+// Returns the sum over the row; the row has an available expert.
 template <int V>
-__device__ __forceinline__ void choose_by_logit(const float (&x)[V], int top_k, int lane, int& expert, float& logit) {
-  unsigned key[V];
+__device__ __forceinline__ float row_shares(const float (&x)[V], bool sigmoid, float top, float (&h)[V],
+                                            float (&rest)[V]) {
+  float sum = 0.0f;
+  if (!sigmoid) {
+    const float c = top * kLog2E;
+    if (fabsf(top) < kHuge) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) key[j] = x[j] > -INFINITY ? ordered(x[j]) : 0u;
-  expert = -1;
-  logit = 0.0f;
-  for (int k = 0; k < top_k; ++k) {
-    unsigned best = 0;
-    int at = 0;
+      for (int j = 0; j < V; ++j) { h[j] = power_of_2(fmaf(x[j], kLog2E, -c)); sum += h[j]; }
+    } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (key[j] > best) { best = key[j]; at = j; }
-    const unsigned most = __reduce_max_sync(kAll, best);
-    if (most == 0) break;
-    const unsigned e = __reduce_min_sync(kAll, best == most ? at * 32 + lane : 0x7fffffffu);
-    if (lane == k) { expert = static_cast<int>(e); logit = unordered(most); }
+      for (int j = 0; j < V; ++j) { h[j] = exp_below(x[j], top); sum += h[j]; }
+    }
+  } else if (top > kFar) {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j * 32 + lane == static_cast<int>(e)) key[j] = 0;
+    for (int j = 0; j < V; ++j) { h[j] = sigmoid_of(x[j], rest[j]); sum += h[j]; }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) { h[j] = sigmoid_far(x[j], top); rest[j] = 1.0f; sum += h[j]; }
   }
+  return warp_sum(sum);
 }
 
-// The same on s + bias.  Scores and their sums with the bias are taken in 64 bits: two experts whose 32-bit
-// values are equal or swapped by a rounding would otherwise come out in another order than their scores have.
-template <int V>
-__device__ __forceinline__ void choose_by_score(const float (&x)[V], const Rows& a, float top, int lane, int& expert,
-                                                float& logit) {
-  double s[V];
-  double sum = 0.0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    s[j] = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x[j]))) : exp(static_cast<double>(x[j]) - top);
-    sum += s[j];
+// The choice of one row from memory, in K rounds over all experts, by 64-bit scores: for rows with too many candidates
+// (more than 32 equal values).  Out of line and without arrays it costs the other rows no registers.
+template <class T>
+__device__ __noinline__ int choose_slowly(const T* logits, int experts, int top_k, const float* bias, bool sigmoid,
+                                          float top, int lane) {
+  double sum = 1.0;
+  if (bias != nullptr && !sigmoid) {
+    sum = 0.0;
+    for (int e = lane; e < experts; e += 32) sum += exp(static_cast<double>(as_float(logits[e])) - top);
+    sum = warp_sum(sum);
   }
-  sum = warp_sum(sum);
-  unsigned long long key[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int e = j * 32 + lane;
-    key[j] = x[j] > -INFINITY
-                 ? ordered((a.sigmoid ? s[j] : s[j] / sum) + static_cast<double>(__ldg(a.bias + e))) : 0ull;
-  }
-  expert = -1;
-  logit = 0.0f;
-  for (int k = 0; k < a.top_k; ++k) {
+  unsigned long long last = ~0ull;   // the order so far ends at (last, last_expert)
+  int last_expert = -1, expert = -1;
+  for (int k = 0; k < top_k; ++k) {
     unsigned long long best = 0;
-    int at = 0;
-    float its = 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (key[j] > best) { best = key[j]; at = j; its = x[j]; }
+    int at = 0x7fffffff;
+    for (int e = lane; e < experts; e += 32) {
+      const double x = as_float(logits[e]);
+      if (!(x > -INFINITY)) continue;
+      double v = x;
+      if (bias != nullptr) v = (sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum) + static_cast<double>(__ldg(bias + e));
+      const unsigned long long key = ordered(v);
+      if ((key < last || (key == last && e > last_expert)) && key > best) { best = key; at = e; }
+    }
     const unsigned high = static_cast<unsigned>(best >> 32), low = static_cast<unsigned>(best);
     const unsigned most_high = __reduce_max_sync(kAll, high);
     if (most_high == 0) break;
     const unsigned most_low = __reduce_max_sync(kAll, high == most_high ? low : 0u);
-    const bool mine = high == most_high && low == most_low;
-    const unsigned e = __reduce_min_sync(kAll, mine ? at * 32 + lane : 0x7fffffffu);
-    const float v = __shfl_sync(kAll, its, e & 31);
-    if (lane == k) { expert = static_cast<int>(e); logit = v; }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j * 32 + lane == static_cast<int>(e)) key[j] = 0;
+    last_expert = __reduce_min_sync(kAll, high == most_high && low == most_low ? static_cast<unsigned>(at) : 0x7fffffffu);
+    last = static_cast<unsigned long long>(most_high) << 32 | most_low;
+    if (lane == k) expert = last_expert;
   }
+  return expert;
 }
 
-// Lane k: choice k's weight (its gate without the scale).  stats belong to the whole row.
-__device__ __forceinline__ float choice_weight(const Rows& a, const RowStats& stats, int expert, float logit) {
+// The n <= 32 candidates in `held` (any order), ranked by their 64-bit scores; lane k gets choice k.  A lane takes one
+// candidate, so this costs one exponential in 64 bits (and for softmax the row's sum).
+template <class T>
+__device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, const float* bias, bool sigmoid,
+                                       float top, int lane, float2* held, int n) {
+  double sum = 1.0;
+  if (!sigmoid) {
+    sum = 0.0;
+#pragma unroll 4
+    for (int e = lane; e < experts; e += 32) sum += exp(static_cast<double>(as_float(logits[e])) - top);
+    sum = warp_sum(sum);
+  }
+  int expert = 0x7fffffff;
+  double v = -INFINITY;
+  if (lane < n) {
+    expert = __float_as_int(held[lane].y);
+    const double x = as_float(logits[expert]);
+    v = (sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum) + static_cast<double>(__ldg(bias + expert));
+  }
+  int before = 0;
+  for (int i = 0; i < n; ++i) {
+    const double w = __shfl_sync(kAll, v, i);
+    const int e = __shfl_sync(kAll, expert, i);
+    before += w > v || (w == v && e < expert);
+  }
+  __syncwarp();
+  if (lane < n) held[before].y = __int_as_float(expert);
+  __syncwarp();
+  expert = lane < min(n, top_k) ? __float_as_int(held[lane].y) : -1;
+  __syncwarp();
+  return expert;
+}
+
+// The K largest (value, lowest expert first) of the warp's V x 32 values; -inf is no candidate.  The (K+1)th largest
+// of the lanes' maxima is at most the (K+1)th largest value, so the values from it up hold the choice and the one
+// behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They, and with a margin what is at
+// most so much smaller, are gathered in `held` (32 of this warp), and each counts the ones before it.  Lane k gets choice
+// k and its value; `behind` the next value (-inf: none).  Returns the number of candidates, which stay in `held` in
+// their order; above 32 (many equal values) nothing is chosen.
+template <int V, int VEC>
+__device__ __forceinline__ int choose(const float (&x)[V], float margin, int top_k, int lane, float2* held, int& expert,
+                                      float& its, float& behind) {
+  float most = x[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) most = fmaxf(most, x[j]);
+  unsigned key = most > -INFINITY ? ordered(most) : 0u, border = 0;
+  for (int k = 0; k <= top_k; ++k) {   // equal maxima go at once: the border is then lower, which is as good
+    border = __reduce_max_sync(kAll, key);
+    if (border == 0) break;
+    if (key == border) key = 0;
+  }
+  float from = -FLT_MAX;
+  if (border != 0) from = unordered(border) - margin * (1.0f + fabsf(unordered(border)));
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mine += x[j] >= from;
+  // places: lanes before this one with at least 1, 2, ... candidates
+  int at = 0, n = 0;
+  const unsigned before_me = (1u << lane) - 1;
+  for (int c = 1;; ++c) {
+    const unsigned lanes = __ballot_sync(kAll, mine >= c);
+    if (lanes == 0) break;
+    at += __popc(lanes & before_me);
+    n += __popc(lanes);
+  }
+  if (n > 32) return n;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (x[j] >= from) held[at++] = make_float2(x[j], __int_as_float(expert_of<VEC>(j, lane)));
+  __syncwarp();
+  float2 me = make_float2(-INFINITY, __int_as_float(0x7fffffff));
+  if (lane < n) me = held[lane];
+  int before = 0;
+  for (int i = 0; i < n; ++i) {
+    const float2 other = held[i];
+    before += other.x > me.x || (other.x == me.x && __float_as_int(other.y) < __float_as_int(me.y));
+  }
+  __syncwarp();
+  if (lane < n) held[before] = me;
+  __syncwarp();
+  expert = -1;
+  its = -INFINITY;
+  if (lane < min(n, top_k)) {
+    const float2 w = held[lane];
+    its = w.x;
+    expert = __float_as_int(w.y);
+  }
+  behind = n > top_k ? held[top_k].x : -INFINITY;
+  __syncwarp();
+  return n;
+}
+
+// The choice by s + bias.  In 32 bits v = s + bias is off by less than doubt * (1 + |v|): a sigmoid by 9 half units
+// (exponential 4, addition 1, reciprocal 2, product 1, and the residual), a softmax by 46 (0.37 for the difference,
+// exponential 4, 37 additions, reciprocal and product), and v by its own rounding.  Where two neighbours of the
+// order, or the last choice and the one behind it, are nearer than twice that, 64 bits decide among the candidates
+// (0.3 % of rows for sigmoids of 512 experts).  Experts of equal logit and equal bias have equal scores and need no more
+// digits.  False: too many candidates, nothing is chosen.
+template <class T, int V, int VEC>
+__device__ __forceinline__ bool choose_by_score(const float (&x)[V], const float (&h)[V], float sum, const Rows& a,
+                                                const T* logits, float top, int lane, float2* held, int& expert) {
+  const float doubt = a.sigmoid ? 1e-6f : 4e-6f;
+  float v[V];
+  const float inv = a.sigmoid ? 1.0f : reciprocal(sum);
+#pragma unroll
+  for (int j = 0; j < V; j += VEC) {
+    const int e = expert_of<VEC>(j, lane);
+    const bool there = e < a.experts;
+#pragma unroll
+    for (int i = 0; i < VEC; i += VEC % 4 == 0 ? 4 : 1) {
+      float bias[4] = {};
+      if (there) {
+        if constexpr (VEC % 4 == 0) *reinterpret_cast<float4*>(bias) = __ldg(reinterpret_cast<const float4*>(a.bias + e + i));
+        else bias[0] = __ldg(a.bias + e + i);
+      }
+#pragma unroll
+      for (int w = 0; w < (VEC % 4 == 0 ? 4 : 1); ++w) {
+        const int at = j + i + w;
+        const float s = a.sigmoid && top <= kFar ? 0.0f : h[at] * inv;   // sigmoids of such a row are below 1e-26
+        v[at] = x[at] > -INFINITY ? s + bias[w] : -INFINITY;
+      }
+    }
+  }
+  float mine, behind;
+  const int n = choose<V, VEC>(v, 2.0f * doubt, a.top_k, lane, held, expert, mine, behind);
+  if (n > 32) return false;
+  float next = __shfl_down_sync(kAll, mine, 1);
+  int next_expert = __shfl_down_sync(kAll, expert, 1);
+  if (lane >= a.top_k - 1) { next = behind; next_expert = -1; }
+  bool doubtful = false;
+  if (expert >= 0 && next > -INFINITY && !(mine - next > 2.0f * doubt * (1.0f + fabsf(mine)))) {
+    doubtful = true;
+    if (next_expert >= 0)
+      doubtful = as_float(logits[expert]) != as_float(logits[next_expert]) ||
+                 __ldg(a.bias + expert) != __ldg(a.bias + next_expert);
+  }
+  if (__any_sync(kAll, doubtful))
+    expert = rank_in_64<T>(logits, a.experts, a.top_k, a.bias, a.sigmoid != 0, top, lane, held, n);
+  return true;
+}
+
+// Lane k: choice k's weight (its gate without the scale).  top and sum belong to the whole row; sum is that of
+// exp(x - top) and is used by softmax without renormalisation alone.
+__device__ __forceinline__ float choice_weight(const Rows& a, float top, float sum, int expert, float logit) {
   const bool chosen = expert >= 0;
+  float rest;
   if (a.renormalize) {
-    const float top = warp_max(chosen ? logit : -INFINITY);
+    const float most = warp_max(chosen ? logit : -INFINITY);
     float h = 0.0f;
-    if (chosen) h = a.sigmoid ? sigmoid_hat(logit, top) : expf(logit - top);
-    const float sum = warp_sum(h);
-    return chosen ? h / sum : 0.0f;
+    if (chosen) h = !a.sigmoid ? exp_below(logit, most) : most > kFar ? sigmoid_of(logit, rest) : sigmoid_far(logit, most);
+    const float all = warp_sum(h);
+    return chosen ? h / all : 0.0f;
   }
   if (!chosen) return 0.0f;
-  return a.sigmoid ? sigmoid_hat(logit, 0.0f) : expf(logit - stats.top) / stats.sum;
+  return a.sigmoid ? sigmoid_of(logit, rest) : exp_below(logit, top) / sum;
 }
 
 // Records of the balance sums: record (chunk c, sequence b) is number c + b.  Chunks and sequences both walk the
@@ -236,20 +414,30 @@ struct Records {
   unsigned* ticket;
 };
 
-template <class T, int V>
-__global__ void __launch_bounds__(kWarps * 32)
+// Blocks of an SM that the registers are shared out for.
+template <int V>
+constexpr int kResident = V <= 8 ? 4 : V <= 16 ? 2 : 1;
+
+template <class T, int V, int VEC>
+__global__ void __launch_bounds__(kWarps * 32, kResident<V>)
 router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict__ gates, const Records rec) {
   extern __shared__ float smem[];
   float* part = smem;                                              // [kWarps][experts]
   int* seen = reinterpret_cast<int*>(smem + kWarps * a.experts);   // [experts]
   __shared__ int live_rows[kWarps], live_routes[kWarps];
+  __shared__ float2 held[kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool balance = rec.share != nullptr, choose = routes != nullptr;
-  if (balance && blockIdx.x == 0 && threadIdx.x == 0) *rec.ticket = 0;   // for the kernel that sums the records
+  const bool balance = rec.share != nullptr, pick = routes != nullptr;
+  const bool whole = balance || a.bias != nullptr || (!a.renormalize && !a.sigmoid);   // scores of all experts
+  if (balance) {
+    cudaTriggerProgrammaticLaunchCompletion();   // the kernel that sums the records may take its place; it waits for these
+    if (blockIdx.x == 0 && threadIdx.x == 0) *rec.ticket = 0;
+  }
   const int first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.tokens);
-  if (balance)
+  if (balance) {
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) seen[e] = 0;
-  __syncthreads();
+    __syncthreads();
+  }
 
   int row0 = first;
   while (row0 < last) {
@@ -260,40 +448,57 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
     int rows = 0, taken = 0;
     for (int row = row0 + warp; row < row1; row += kWarps) {
-      float x[V], h[V];
-      const bool live = row_live(a, row, balance ? b : sequence_of(a, row));
       int expert = -1;
       float weight = 0.0f;
-      if (live) {
-        load_row<T, V>(a, row, lane, x);
-        const RowStats stats = row_stats<V>(x, a.sigmoid, h);
-        if (choose) {
-          float logit = 0.0f;
-          if (stats.bad) {   // no distribution: valid routes and NaN gates, so that it shows in the output
-            expert = lane < a.top_k ? lane : -1;
-            weight = NAN;
+      if (row_live(a, row, balance ? b : sequence_of(a, row))) {
+        float x[V], h[V], rest[V];
+        load_row<T, V, VEC>(a, row, lane, x);
+        const RowTop r = row_top<V>(x, a.sigmoid);
+        float sum = 1.0f;
+        if (whole && r.any && !r.bad) sum = row_shares<V>(x, a.sigmoid, r.top, h, rest);
+        if (balance && (r.any || r.bad)) {
+          ++rows;
+          if (r.bad) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = NAN;
           } else {
-            if (a.bias != nullptr) choose_by_score<V>(x, a, stats.top, lane, expert, logit);
-            else choose_by_logit<V>(x, a.top_k, lane, expert, logit);
-            weight = choice_weight(a, stats, expert, logit);
+            const float inv = 1.0f / sum;
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = fmaf(h[j], inv, acc[j]);
           }
         }
-        if (balance && (stats.any || stats.bad)) {
-          ++rows;
-#pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] += stats.bad ? NAN : h[j] / stats.sum;
-          if (choose && expert >= 0) { atomicAdd(seen + expert, 1); ++taken; }
+        if (pick && r.bad) {   // no distribution: valid routes and NaN gates, so that it shows in the output
+          expert = lane < a.top_k ? lane : -1;
+          weight = NAN;
+        } else if (pick && r.any) {
+          const T* logits = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.stride;
+          float logit = 0.0f, behind;
+          bool settled;
+          if (a.bias != nullptr) {
+            settled = choose_by_score<T, V, VEC>(x, h, sum, a, logits, r.top, lane, held[warp], expert);
+            if (settled && expert >= 0) logit = as_float(logits[expert]);
+          } else {
+            settled = choose<V, VEC>(x, 0.0f, a.top_k, lane, held[warp], expert, logit, behind) <= 32;
+          }
+          if (!settled) {
+            expert = choose_slowly<T>(logits, a.experts, a.top_k, a.bias, a.sigmoid != 0, r.top, lane);
+            if (expert >= 0) logit = as_float(logits[expert]);
+          }
+          weight = choice_weight(a, r.top, sum, expert, logit);
         }
+        if (balance && pick && expert >= 0) { atomicAdd(seen + expert, 1); ++taken; }
       }
-      if (choose && lane < a.top_k) {
+      if (pick && lane < a.top_k) {
         routes[static_cast<long long>(row) * a.top_k + lane] = expert;
         gates[static_cast<long long>(row) * a.top_k + lane] = expert >= 0 ? a.scale * weight : 0.0f;
       }
     }
     if (balance) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j * 32 + lane < a.experts) part[warp * a.experts + j * 32 + lane] = acc[j];
+      for (int j = 0; j < V; ++j) {
+        const int e = expert_of<VEC>(j, lane);
+        if (e < a.experts) part[warp * a.experts + e] = acc[j];
+      }
       taken = __reduce_add_sync(kAll, taken);
       if (lane == 0) { live_rows[warp] = rows; live_routes[warp] = taken; }
       __syncthreads();
@@ -304,7 +509,7 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) sum += part[w * a.experts + e];
           rec.share[record * a.experts + e] = sum;
-          if (choose) { rec.counts[record * a.experts + e] = seen[e]; seen[e] = 0; }
+          if (pick) { rec.counts[record * a.experts + e] = seen[e]; seen[e] = 0; }
         }
         if (threadIdx.x == 0) {
           int n = 0, c = 0;
@@ -319,53 +524,61 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
   }
 }
 
-// Sums the records of one sequence for 32 experts per block (8 warps take every eighth record), then the last
+// Sums the records of one sequence for 32 experts per block (32 warps take every 32nd record), then the last
 // block to finish sums the blocks' parts of the loss in their order.
 // table: [num_sequences][experts] of (f - 1) / n_b, the loss's slope by p up to a constant (p sums to one, so a
 // constant drops out of the gradient; without it the differences near f = 1 keep their digits), then 1 / live sequences.
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kFinishWarps * 32)
 balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ given, int* __restrict__ counts,
                       float* __restrict__ table, float* parts, float* __restrict__ loss) {
-  __shared__ float share[kWarps][32];
-  __shared__ int count[kWarps][32];
-  __shared__ int rows[kWarps], taken[kWarps];
+  __shared__ float share[kFinishWarps][32];
+  __shared__ int count[kFinishWarps][32];
+  __shared__ int rows[kFinishWarps], taken[kFinishWarps];
+  __shared__ long long given_sum[kFinishWarps];
   __shared__ bool is_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y, e = blockIdx.x * 32 + lane;
+  cudaGridDependencySynchronize();   // launched while the kernel that writes the records still runs
   const int row0 = a.sequences == nullptr ? 0 : max(0, __ldg(a.sequences + b));
   const int row1 = sequence_end(a, b);
   float sum = 0.0f;
   int c = 0, n = 0, total = 0;
   if (row0 < row1) {
-    for (int chunk = row0 / a.chunk + warp; chunk <= (row1 - 1) / a.chunk; chunk += kWarps) {
-      const long long record = chunk + b;
-      if (e < a.experts) {
-        sum += rec.share[record * a.experts + e];
-        if (rec.counts != nullptr) c += rec.counts[record * a.experts + e];
+    const int end = (row1 - 1) / a.chunk;
+    if (e < a.experts) {
+#pragma unroll 8
+      for (int chunk = row0 / a.chunk + warp; chunk <= end; chunk += kFinishWarps) {
+        const long long at = static_cast<long long>(chunk + b) * a.experts + e;
+        sum += rec.share[at];
+        if (rec.counts != nullptr) c += rec.counts[at];
       }
-      n += rec.rows[2 * record];
-      total += rec.rows[2 * record + 1];
+    }
+    for (int chunk = row0 / a.chunk + threadIdx.x; chunk <= end; chunk += blockDim.x) {
+      n += rec.rows[2 * static_cast<long long>(chunk + b)];
+      total += rec.rows[2 * static_cast<long long>(chunk + b) + 1];
     }
   }
+  long long all = 0;
+  if (given != nullptr)
+    for (int i = threadIdx.x; i < a.experts; i += blockDim.x) all += given[static_cast<long long>(b) * a.experts + i];
   share[warp][lane] = sum;
   count[warp][lane] = c;
-  if (lane == 0) { rows[warp] = n; taken[warp] = total; }
+  n = __reduce_add_sync(kAll, n);
+  total = __reduce_add_sync(kAll, total);
+  all = warp_sum(all);
+  if (lane == 0) { rows[warp] = n; taken[warp] = total; given_sum[warp] = all; }
   __syncthreads();
   if (warp == 0) {
     sum = 0.0f;
-    c = n = 0;
-    long long all = 0;
-    for (int w = 0; w < kWarps; ++w) { sum += share[w][lane]; c += count[w][lane]; n += rows[w]; all += taken[w]; }
-    if (given != nullptr) {
-      all = 0;
-      for (int i = lane; i < a.experts; i += 32) all += given[static_cast<long long>(b) * a.experts + i];
+    c = 0;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(kAll, all, d);
-      c = e < a.experts ? given[static_cast<long long>(b) * a.experts + e] : 0;
-    }
-    float f = 0.0f, part = 0.0f;
+    for (int w = 0; w < kFinishWarps; ++w) { sum += share[w][lane]; c += count[w][lane]; }
+    n = __reduce_add_sync(kAll, rows[lane]);
+    all = warp_sum(given != nullptr ? given_sum[lane] : static_cast<long long>(taken[lane]));
+    if (given != nullptr) c = e < a.experts ? given[static_cast<long long>(b) * a.experts + e] : 0;
+    float part = 0.0f;
     if (e < a.experts) {
-      f = all > 0 ? static_cast<float>(static_cast<double>(c) * a.experts / static_cast<double>(all)) : 0.0f;
+      const float f = all > 0 ? static_cast<float>(static_cast<double>(c) * a.experts / static_cast<double>(all)) : 0.0f;
       const float inv = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
       part = n > 0 ? f * (sum / static_cast<float>(n)) : 0.0f;
       table[static_cast<long long>(b) * a.experts + e] = (f - 1.0f) * inv;
@@ -383,7 +596,7 @@ balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ g
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  __shared__ double sums[kWarps], lives[kWarps];
+  __shared__ double sums[kFinishWarps], lives[kFinishWarps];
   double l = 0.0, live = 0.0;
   const long long blocks = static_cast<long long>(gridDim.x) * gridDim.y;
   for (long long i = threadIdx.x; i < blocks; i += blockDim.x) { l += __ldcg(parts + 2 * i); live += __ldcg(parts + 2 * i + 1); }
@@ -391,12 +604,14 @@ balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ g
   live = warp_sum(live);
   if (lane == 0) { sums[warp] = l; lives[warp] = live; }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    l = live = 0.0;
-    for (int w = 0; w < kWarps; ++w) { l += sums[w]; live += lives[w]; }
-    const double inv = live > 0.0 ? 1.0 / live : 0.0;
-    *loss = static_cast<float>(live > 0.0 ? l * inv : 0.0);
-    table[static_cast<long long>(a.num_sequences) * a.experts] = static_cast<float>(inv);
+  if (warp == 0) {
+    l = warp_sum(sums[lane]);
+    live = warp_sum(lives[lane]);
+    if (lane == 0) {
+      const double inv = live > 0.0 ? 1.0 / live : 0.0;
+      *loss = static_cast<float>(live > 0.0 ? l * inv : 0.0);
+      table[static_cast<long long>(a.num_sequences) * a.experts] = static_cast<float>(inv);
+    }
   }
 }
 
@@ -405,88 +620,139 @@ balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ g
 //     softmax, renormalised  w_k (g_k - sum w g) at the chosen      softmax  s_e ([chosen] g_e - sum s g)
 //     sigmoid, renormalised  (1 - s_k) w_k (g_k - sum w g)           sigmoid  (1 - s_k) s_k g_k
 //   loss, q = the table's row times dloss / live sequences:  p_e (q_e - sum p q), times 1 - s_e for sigmoid.
-template <class T, int V>
-__global__ void __launch_bounds__(kWarps * 32)
+// The choices' part goes through a row of shared memory that is zero between rows.  A warp takes a.chunk rows in a row.
+template <class T, int V, int VEC>
+__global__ void __launch_bounds__(kWarps * 32, kResident<V>)
 router_backward_kernel(const Rows a, const int* __restrict__ routes, const float* __restrict__ dgates,
                        const float* __restrict__ table, const float* __restrict__ dloss, T* __restrict__ dlogits) {
+  extern __shared__ float4 smem_rows[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* chosen = reinterpret_cast<float*>(smem_rows) + warp * (V * 32);
   const float push = table != nullptr
       ? __ldg(dloss) * __ldg(table + static_cast<long long>(a.num_sequences) * a.experts) : 0.0f;
-  for (long long r = static_cast<long long>(blockIdx.x) * kWarps + warp; r < a.tokens;
-       r += static_cast<long long>(gridDim.x) * kWarps) {
-    const int row = static_cast<int>(r);
-    const int b = sequence_of(a, row);
-    float x[V], h[V], d[V];
+  const bool shares = table != nullptr || (!a.renormalize && !a.sigmoid);
+  if (routes != nullptr) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) chosen[j * 32 + lane] = 0.0f;
+    __syncwarp();
+  }
+  const long long from = (static_cast<long long>(blockIdx.x) * kWarps + warp) * a.chunk;
+  const int end = static_cast<int>(min(from + a.chunk, static_cast<long long>(a.tokens)));
+  int b = 0, b_end = -1;
+  for (int row = static_cast<int>(min(from, static_cast<long long>(a.tokens))); row < end; ++row) {
+    if (row >= b_end) {
+      b = sequence_of(a, row);
+      b_end = max(row + 1, sequence_end(a, b));
+    }
+    float d[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.0f;
     if (row_live(a, row, b)) {
-      load_row<T, V>(a, row, lane, x);
-      const RowStats stats = row_stats<V>(x, a.sigmoid, h);
-      if (stats.bad) {
+      int expert = -1;
+      float logit = 0.0f, g = 0.0f;
+      if (routes != nullptr && lane < a.top_k) {
+        const long long at = static_cast<long long>(row) * a.top_k + lane;
+        expert = routes[at];
+        if (static_cast<unsigned>(expert) >= static_cast<unsigned>(a.experts)) expert = -1;
+        g = a.scale * dgates[at];
+        if (expert >= 0) logit = as_float((static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.stride)[expert]);
+      }
+      float x[V], h[V], rest[V];
+      load_row<T, V, VEC>(a, row, lane, x);
+      const RowTop r = row_top<V>(x, a.sigmoid);
+      if (r.bad) {
 #pragma unroll
         for (int j = 0; j < V; ++j) d[j] = NAN;
-      } else if (stats.any) {
-        const float inv = 1.0f / stats.sum;
+      } else if (r.any) {
+        float sum = 1.0f;
+        if (shares) sum = row_shares<V>(x, a.sigmoid, r.top, h, rest);
+        const float inv = 1.0f / sum;
         if (table != nullptr) {
           const float* q = table + static_cast<long long>(b) * a.experts;
-          float mean = 0.0f, w[V];
+          float mean = 0.0f;
+          constexpr int kWide = VEC % 4 == 0 ? 4 : 1;   // then experts % 4 == 0, and every row of the table is aligned
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int e = j * 32 + lane;
-            w[j] = e < a.experts ? __ldg(q + e) : 0.0f;
-            h[j] *= inv;
-            mean = fmaf(h[j], w[j], mean);
-          }
-          mean = warp_sum(mean);
+          for (int j = 0; j < V; j += kWide) {
+            const int e = expert_of<VEC>(j, lane);
+            Piece<float, kWide> w{};
+            if (e < a.experts) w = *reinterpret_cast<const Piece<float, kWide>*>(q + e);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            d[j] = push * h[j] * (w[j] - mean);
-            if (a.sigmoid) d[j] *= sigmoid_rest(x[j]);
-          }
-        }
-        if (routes != nullptr) {
-          int expert = -1;
-          float logit = 0.0f, g = 0.0f;
-          if (lane < a.top_k) {
-            expert = routes[r * a.top_k + lane];
-            if (static_cast<unsigned>(expert) >= static_cast<unsigned>(a.experts)) expert = -1;
-            if (expert >= 0) {
-              logit = as_float((static_cast<const T*>(a.logits) + r * a.stride)[expert]);
-              g = a.scale * dgates[r * a.top_k + lane];
+            for (int i = 0; i < kWide; ++i) {
+              d[j + i] = w.v[i];
+              mean = fmaf(h[j + i], w.v[i], mean);
             }
           }
-          const float w = choice_weight(a, stats, expert, logit);
+          mean = warp_sum(mean) * inv;
+          const float factor = push * inv;
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] = (factor * (a.sigmoid ? h[j] * rest[j] : h[j])) * (d[j] - mean);
+        }
+        if (routes != nullptr) {
+          const float w = choice_weight(a, r.top, sum, expert, logit);
           float mean = 0.0f;
           if (a.renormalize || !a.sigmoid) mean = warp_sum(w * g);
           float c = w * (a.renormalize ? g - mean : g);
-          if (a.sigmoid) c *= sigmoid_rest(logit);
+          if (a.sigmoid) {
+            float rest_k;
+            sigmoid_of(logit, rest_k);
+            c *= logit > kFar ? rest_k : 1.0f;
+          }
           if (!a.renormalize && !a.sigmoid) {
-            const float factor = table != nullptr ? mean : mean * inv;   // h holds shares when the loss ran first
 #pragma unroll
-            for (int j = 0; j < V; ++j) d[j] -= h[j] * factor;
+            for (int j = 0; j < V; ++j) d[j] = fmaf(h[j], -mean * inv, d[j]);
           }
-          for (int k = 0; k < a.top_k; ++k) {
-            const int e = __shfl_sync(kAll, expert, k);
-            const float v = __shfl_sync(kAll, c, k);
-            if (e >= 0 && (e & 31) == lane) {
+          if (expert >= 0) chosen[expert] = c;
+          __syncwarp();
 #pragma unroll
-              for (int j = 0; j < V; ++j)
-                if (j == e >> 5) d[j] += v;
-            }
+          for (int j = 0; j < V; j += VEC) {
+            const Piece<float, VEC> piece = *reinterpret_cast<const Piece<float, VEC>*>(chosen + expert_of<VEC>(j, lane));
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) d[j + i] += piece.v[i];
           }
+          __syncwarp();
+          if (expert >= 0) chosen[expert] = 0.0f;
+          __syncwarp();
         }
       }
     }
-    T* out = dlogits + r * a.experts;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = j * 32 + lane;
-      if (e < a.experts) put(out + e, d[j]);
-    }
+    store_row<T, V, VEC>(dlogits + static_cast<long long>(row) * a.experts, a.experts, lane, d);
   }
 }
 
-// Routes per expert: a block counts its rows in shared memory and adds the whole numbers to the result.
+// Routes per expert of one sequence by a cluster of eight CTAs: each counts an eighth of the rows in its shared memory
+// and sums a share of the experts over all eight.  Nothing has to be cleared before.
+constexpr int kCountCtas = 8;
+__global__ void __cluster_dims__(kCountCtas, 1, 1) __launch_bounds__(1024)
+expert_counts_cluster_kernel(const Rows a, const int* __restrict__ routes, int* __restrict__ counts) {
+  extern __shared__ int cluster_counts[];
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) cluster_counts[e] = 0;
+  __syncthreads();
+  const int b = blockIdx.y, part = blockIdx.x;
+  const int row0 = a.sequences == nullptr ? 0 : max(0, __ldg(a.sequences + b));
+  const long long rows = max(0, sequence_end(a, b) - row0);
+  const long long first = (row0 + rows * part / kCountCtas) * a.top_k;
+  const long long last = (row0 + rows * (part + 1) / kCountCtas) * a.top_k;
+  for (long long i = first + threadIdx.x; i < last; i += blockDim.x) {
+    const int e = routes[i];
+    if (static_cast<unsigned>(e) < static_cast<unsigned>(a.experts)) atomicAdd(cluster_counts + e, 1);
+  }
+  cluster_sync_all();
+  for (int e = part * blockDim.x + threadIdx.x; e < a.experts; e += kCountCtas * blockDim.x) {
+    const uint32_t at = smem_u32(cluster_counts + e);
+    int c = 0;
+#pragma unroll
+    for (int s = 0; s < kCountCtas; ++s) {
+      int v;
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(map_to_cta(at, s)) : "memory");
+      c += v;
+    }
+    counts[static_cast<long long>(b) * a.experts + e] = c;
+  }
+  cluster_sync_all();   // the others' shared memory stays until it is read
+}
+
+// For many routes, or many sequences: a block counts its rows in shared memory and adds the whole numbers to the
+// (cleared) result.
 __global__ void __launch_bounds__(256)
 expert_counts_kernel(const Rows a, const int* __restrict__ routes, int* __restrict__ counts) {
   extern __shared__ int seen_counts[];
@@ -516,6 +782,10 @@ expert_counts_kernel(const Rows a, const int* __restrict__ routes, int* __restri
 }
 
 // ------------------------------------------------------------------ host side
+// Up to here one cluster a sequence is the quicker form of the counts (one launch instead of a clear and a launch).
+constexpr int kClusterSequences = 32;
+constexpr long long kClusterRoutes = 131072;
+
 struct Plan {
   int chunk, blocks;
   long long records, parts;
@@ -525,7 +795,8 @@ struct Plan {
 Plan plan_of(const wm_router& r) {
   Plan p{};
   const int sequences = r.sequences ? r.num_sequences : 1;
-  const int want = (r.tokens + kWarps - 1) / kWarps;
+  // Two rows a warp where that still gives every SM two blocks: fewer records for the kernel behind this one.
+  const int want = r.tokens >= 2 * 296 * kWarps ? (r.tokens + 2 * kWarps - 1) / (2 * kWarps) : (r.tokens + kWarps - 1) / kWarps;
   const int blocks = want < kMaxBlocks ? (want > 0 ? want : 1) : kMaxBlocks;
   p.chunk = r.tokens > 0 ? (r.tokens + blocks - 1) / blocks : 1;
   p.blocks = r.tokens > 0 ? (r.tokens + p.chunk - 1) / p.chunk : 1;
@@ -569,39 +840,63 @@ Records records_of(const Plan& p, void* workspace, bool counts) {
                  reinterpret_cast<int*>(w + p.rows), reinterpret_cast<unsigned*>(w + p.ticket)};
 }
 
-template <class T, int V>
-int forward_of(const Rows& a, const Plan& p, int* routes, float* gates, const Records& rec, cudaStream_t stream) {
+template <class T, int V, int VEC>
+void forward_of(const Rows& a, const Plan& p, int* routes, float* gates, const Records& rec, cudaStream_t stream) {
   const int smem = rec.share ? (kWarps + 1) * a.experts * 4 : 0;
-  router_forward_kernel<T, V><<<p.blocks, kWarps * 32, smem, stream>>>(a, routes, gates, rec);
-  return 0;
+  router_forward_kernel<T, V, VEC><<<p.blocks, kWarps * 32, smem, stream>>>(a, routes, gates, rec);
 }
-template <class T, int V>
-int backward_of(const Rows& a, const int* routes, const float* dgates, const float* table, const float* dloss,
-                void* dlogits, cudaStream_t stream) {
-  const int want = (a.tokens + kWarps - 1) / kWarps;
-  router_backward_kernel<T, V><<<want < 8 * kMaxBlocks ? want : 8 * kMaxBlocks, kWarps * 32, 0, stream>>>(
-      a, routes, dgates, table, dloss, static_cast<T*>(dlogits));
-  return 0;
+template <class T, int V, int VEC>
+void backward_of(const Rows& a, const int* routes, const float* dgates, const float* table, const float* dloss,
+                 void* dlogits, cudaStream_t stream) {
+  Rows rows = a;
+  const int most = 2 * 148 * 3 * kWarps;   // warps: two rounds of what the SMs hold
+  rows.chunk = (a.tokens + most - 1) / most;
+  const int blocks = (a.tokens + rows.chunk * kWarps - 1) / (rows.chunk * kWarps);
+  const int smem = routes ? kWarps * V * 32 * 4 : 0;
+  router_backward_kernel<T, V, VEC><<<blocks, kWarps * 32, smem, stream>>>(rows, routes, dgates, table, dloss,
+                                                                          static_cast<T*>(dlogits));
 }
 
-// Calls f<T, V>: V slots of 32 experts hold a row.
-#define WM_ROUTER_BY_SIZE(T, experts, f, ...)            \
-  ((experts) <= 32    ? f<T, 1>(__VA_ARGS__)             \
-   : (experts) <= 64  ? f<T, 2>(__VA_ARGS__)             \
-   : (experts) <= 128 ? f<T, 4>(__VA_ARGS__)             \
-   : (experts) <= 256 ? f<T, 8>(__VA_ARGS__)             \
-   : (experts) <= 512 ? f<T, 16>(__VA_ARGS__)            \
-                      : f<T, 32>(__VA_ARGS__))
-#define WM_ROUTER_DISPATCH(dtype, experts, f, ...)                                  \
-  ((dtype) == 0   ? WM_ROUTER_BY_SIZE(__nv_bfloat16, experts, f, __VA_ARGS__)       \
-   : (dtype) == 1 ? WM_ROUTER_BY_SIZE(float, experts, f, __VA_ARGS__)               \
-                  : WM_ROUTER_BY_SIZE(__half, experts, f, __VA_ARGS__))
+// Pieces of 16 bytes (of the lane's whole share, where that is less) when every row starts on one, else single elements.
+template <class T, int V>
+constexpr int kPiece = V < 16 / static_cast<int>(sizeof(T)) ? V : 16 / static_cast<int>(sizeof(T));
+template <class T, int V>
+bool in_pieces(const Rows& a, const void* other) {
+  constexpr int n = kPiece<T, V>;
+  constexpr uintptr_t bytes = n * sizeof(T);
+  if (a.bias && reinterpret_cast<uintptr_t>(a.bias) % 16) return false;   // read with the row's layout
+  return n > 1 && a.experts % n == 0 && a.stride % n == 0 && reinterpret_cast<uintptr_t>(a.logits) % bytes == 0 &&
+         reinterpret_cast<uintptr_t>(other) % bytes == 0;
+}
+// Calls f<T, V, VEC>: V slots of 32 experts hold a row.
+#define WM_ROUTER_WITH(T, V, f, a, other, ...)                                                       \
+  (in_pieces<T, V>(a, other) ? f<T, V, kPiece<T, V>>(a, __VA_ARGS__) : f<T, V, 1>(a, __VA_ARGS__))
+#define WM_ROUTER_BY_SIZE(T, f, a, other, ...)                                       \
+  ((a).experts <= 32    ? WM_ROUTER_WITH(T, 1, f, a, other, __VA_ARGS__)             \
+   : (a).experts <= 64  ? WM_ROUTER_WITH(T, 2, f, a, other, __VA_ARGS__)             \
+   : (a).experts <= 128 ? WM_ROUTER_WITH(T, 4, f, a, other, __VA_ARGS__)             \
+   : (a).experts <= 256 ? WM_ROUTER_WITH(T, 8, f, a, other, __VA_ARGS__)             \
+   : (a).experts <= 512 ? WM_ROUTER_WITH(T, 16, f, a, other, __VA_ARGS__)            \
+                        : WM_ROUTER_WITH(T, 32, f, a, other, __VA_ARGS__))
+#define WM_ROUTER_DISPATCH(dtype, f, a, other, ...)                                  \
+  ((dtype) == 0   ? WM_ROUTER_BY_SIZE(__nv_bfloat16, f, a, other, __VA_ARGS__)       \
+   : (dtype) == 1 ? WM_ROUTER_BY_SIZE(float, f, a, other, __VA_ARGS__)               \
+                  : WM_ROUTER_BY_SIZE(__half, f, a, other, __VA_ARGS__))
 
 int finish(const Rows& a, const Plan& p, const Records& rec, const int* given, int* counts, float* table,
            void* workspace, float* loss, cudaStream_t stream) {
   const dim3 grid((a.experts + 31) / 32, a.num_sequences);
-  balance_finish_kernel<<<grid, kWarps * 32, 0, stream>>>(
-      a, rec, given, counts, table, reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part), loss);
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(kFinishWarps * 32);
+  config.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  WM_CUDA(cudaLaunchKernelEx(&config, balance_finish_kernel, a, rec, given, counts, table,
+                             reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part), loss));
   count_launch();
   WM_CUDA(cudaGetLastError());
   return WM_OK;
@@ -633,7 +928,7 @@ extern "C" int wm_router_forward(const wm_router* r, int32_t* routes, float* gat
   const Rows a = rows_of(*r, p);
   const Records rec = balance ? records_of(p, workspace, true) : Records{};
   // with no rows the kernel still clears the ticket of the kernel behind it
-  WM_ROUTER_DISPATCH(r->dtype, r->experts, forward_of, a, p, routes, gates, rec, stream);
+  WM_ROUTER_DISPATCH(r->dtype, forward_of, a, nullptr, p, routes, gates, rec, stream);
   count_launch();
   WM_CUDA(cudaGetLastError());
   return balance ? finish(a, p, rec, nullptr, counts, table, workspace, loss, stream) : WM_OK;
@@ -654,7 +949,7 @@ extern "C" int wm_balance_forward(const wm_router* r, const int32_t* counts, flo
   const Records rec = records_of(p, workspace, false);
   int* no_routes = nullptr;
   float* no_gates = nullptr;
-  WM_ROUTER_DISPATCH(r->dtype, r->experts, forward_of, a, p, no_routes, no_gates, rec, stream);
+  WM_ROUTER_DISPATCH(r->dtype, forward_of, a, nullptr, p, no_routes, no_gates, rec, stream);
   count_launch();
   WM_CUDA(cudaGetLastError());
   return finish(a, p, rec, counts, nullptr, table, workspace, loss, stream);
@@ -673,7 +968,7 @@ extern "C" int wm_router_backward(const wm_router* r, const int32_t* routes, con
   if (r->tokens == 0) return WM_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const Rows a = rows_of(*r, plan_of(*r));
-  WM_ROUTER_DISPATCH(r->dtype, r->experts, backward_of, a, routes, dgates, table, dloss, dlogits, stream);
+  WM_ROUTER_DISPATCH(r->dtype, backward_of, a, dlogits, routes, dgates, table, dloss, dlogits, stream);
   count_launch();
   WM_CUDA(cudaGetLastError());
   return WM_OK;
@@ -689,16 +984,21 @@ extern "C" int wm_expert_counts(const int32_t* routes, int32_t tokens, int32_t t
   }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const int rows = sequences ? num_sequences : 1;
-  WM_CUDA(cudaMemsetAsync(counts, 0, static_cast<size_t>(rows) * experts * 4, stream));
-  if (tokens == 0) return WM_OK;
-  const int want = (tokens + 127) / 128;
-  const int blocks = want < 296 ? want : 296;
   Rows a{};
   a.tokens = tokens;
   a.experts = experts;
   a.top_k = top_k;
   a.sequences = sequences;
   a.num_sequences = rows;
+  if (rows <= kClusterSequences && static_cast<long long>(tokens) * top_k <= kClusterRoutes) {
+    expert_counts_cluster_kernel<<<dim3(kCountCtas, rows), 1024, experts * 4, stream>>>(a, routes, counts);
+    count_launch();
+    WM_CUDA(cudaGetLastError());
+    return WM_OK;
+  }
+  WM_CUDA(cudaMemsetAsync(counts, 0, static_cast<size_t>(rows) * experts * 4, stream));
+  const int want = (tokens + 127) / 128;
+  const int blocks = want < 296 ? want : 296;
   a.chunk = (tokens + blocks - 1) / blocks;
   expert_counts_kernel<<<(tokens + a.chunk - 1) / a.chunk, 256, experts * 4, stream>>>(a, routes, counts);
   count_launch();

@@ -20,9 +20,9 @@ import weakref
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._launch import on_device, stream_of
 
 _BLOCK_K = 128
 _SOURCE_DTYPES = (torch.bfloat16, torch.float32)
@@ -84,10 +84,14 @@ class FP8Tensor:
         return (self.data.float() * per_elem)[..., :k]
 
 
-def _allocate(shape, block_rows, device) -> FP8Tensor:
+def _allocate(shape, block_rows, like) -> FP8Tensor:
+    """Uninitialised storage on the device of `like`; what the constructor checks holds by construction."""
     data_shape, scale_shape = _storage_shapes(shape, block_rows)
-    return FP8Tensor(torch.empty(data_shape, dtype=torch.float8_e4m3fn, device=device),
-                     torch.empty(scale_shape, dtype=torch.float32, device=device), tuple(shape), block_rows)
+    made = object.__new__(FP8Tensor)
+    made.__dict__.update(data=like.new_empty(data_shape, dtype=torch.float8_e4m3fn),
+                         scales=like.new_empty(scale_shape, dtype=torch.float32), shape=tuple(shape),
+                         block_rows=block_rows)
+    return made
 
 
 def _swap_last_two(shape):
@@ -108,12 +112,10 @@ def quantize_fp8(tensor: torch.Tensor, *, block_rows: int = 1, transpose: bool =
     if block_rows not in (1, 128):
         raise ValueError("block_rows must be 1 or 128")
     logical = _swap_last_two(tuple(tensor.shape)) if transpose else tuple(tensor.shape)
-    with torch.cuda.device(tensor.device):
-        out = _allocate(logical, block_rows, tensor.device)
-        stream = torch.cuda.current_stream()
-        _lib.check(_lib.load().wm_fp8_quantize(*_source_args(tensor), block_rows, int(transpose),
-                                               _lib.ptr(out.data), _lib.ptr(out.scales), stream.cuda_stream))
-        tensor.record_stream(stream)
+    with on_device(tensor.device):
+        out = _allocate(logical, block_rows, tensor)
+        _lib.check(_lib.load().wm_fp8_quantize(*_source_args(tensor), block_rows, int(transpose), out.data.data_ptr(),
+                                               out.scales.data_ptr(), stream_of(tensor.device, tensor)))
     return out
 
 
@@ -122,8 +124,8 @@ def _quantize_fp8_weight_pair(tensor: torch.Tensor) -> tuple[FP8Tensor, FP8Tenso
     bytes and the same block scales (reference kernel: src/cuda/fp8/quantization.cuh:157-237)."""
     _require_cuda(tensor, _SOURCE_DTYPES, "weight quantisation")
     with torch.cuda.device(tensor.device):
-        straight = _allocate(tuple(tensor.shape), 128, tensor.device)
-        flipped = _allocate(_swap_last_two(tuple(tensor.shape)), 128, tensor.device)
+        straight = _allocate(tuple(tensor.shape), 128, tensor)
+        flipped = _allocate(_swap_last_two(tuple(tensor.shape)), 128, tensor)
         stream = torch.cuda.current_stream()
         _lib.check(_lib.load().wm_fp8_quantize_weight(
             *_source_args(tensor), _lib.ptr(straight.data), _lib.ptr(straight.scales),
@@ -138,7 +140,7 @@ def transpose_fp8_weight(weight: FP8Tensor) -> FP8Tensor:
         raise ValueError("Rowwise activations require a new columnwise quantization")
     device = weight.data.device
     with torch.cuda.device(device):
-        out = _allocate(_swap_last_two(tuple(weight.shape)), 128, device)
+        out = _allocate(_swap_last_two(tuple(weight.shape)), 128, weight.data)
         stream = torch.cuda.current_stream()
         _lib.check(_lib.load().wm_fp8_transpose_weight(
             _lib.ptr(weight.data), _lib.ptr(weight.scales), weight.batches, weight.shape[-2], weight.shape[-1],
@@ -176,12 +178,6 @@ def fp8_gemm(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Ten
     return out
 
 
-def _keep(stream, *tensors):
-    """Keeps the storage of operands that were made on another stream until this stream has read them."""
-    for t in tensors:
-        t.record_stream(stream)
-
-
 def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Tensor | None = None,
                accumulate: bool = False) -> torch.Tensor:
     """A @ B^T of A [M, K] and B [N, K], blocks of 1 or 128 rows on either side, any scales.
@@ -198,20 +194,18 @@ def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.T
         raise ValueError("FP8 accumulation requires an existing FP32 output")
     (m, k), n = a.shape, b.shape[0]
     device = a.data.device
-    with torch.cuda.device(device):
+    with on_device(device):
         if out is None:
-            out = torch.empty((m, n), dtype=dtype, device=device)
+            out = a.scales.new_empty((m, n), dtype=dtype)
         else:
             fits = (isinstance(out, torch.Tensor) and tuple(out.shape) == (m, n) and out.dtype == dtype
                     and out.device == device and (n <= 1 or out.stride(1) == 1) and (m <= 1 or out.stride(0) >= n))
             if not fits:
                 raise ValueError("FP8 output shape, dtype, device or layout mismatch")
-        stream = torch.cuda.current_stream()
         _lib.check(_lib.load().wm_fp8_matmul(
-            _lib.ptr(a.data), _lib.ptr(a.scales), _lib.ptr(b.data), _lib.ptr(b.scales), _lib.ptr(out),
+            a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(), out.data_ptr(),
             out.stride(0) if m > 1 else max(n, 1), m, n, k, a.block_rows, b.block_rows, int(dtype == torch.float32),
-            int(accumulate), stream.cuda_stream))
-        _keep(stream, a.data, a.scales, b.data, b.scales)
+            int(accumulate), stream_of(device, a.data, a.scales, b.data, b.scales)))
     return out
 
 
@@ -391,9 +385,12 @@ class PreparedFP8Linear:
             self._origin.check(parameter)
 
     def wait(self):
-        """Order the current stream after the preparation kernels."""
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream().wait_event(self._ready)
+        """Order the current stream after the preparation kernels, until they are known to be done."""
+        if self._ready is not None and not torch.cuda.is_current_stream_capturing():
+            if self._ready.query():
+                self._ready = None
+            else:
+                torch.cuda.current_stream().wait_event(self._ready)
 
 
 @torch.inference_mode(False)
@@ -425,8 +422,9 @@ class _FP8Linear(torch.autograd.Function):
         return fp8_matmul(quantize_fp8(x), prepared.weight, dtype=x.dtype)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("The gradients of fp8_linear cannot be differentiated again")
         x, weight = ctx.saved_tensors
         prepared = ctx.prepared
         dx = dweight = None
@@ -457,11 +455,11 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, prepared: PreparedFP8Linea
         raise ValueError("x, weight and the prepared weight do not match in size or device")
     training = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
     prepared.validate(weight, training=training and x.requires_grad)
-    rows = x.reshape(-1, x.shape[-1]).contiguous()
-    with torch.cuda.device(x.device):
+    rows = x if x.ndim == 2 and x.is_contiguous() else x.reshape(-1, x.shape[-1]).contiguous()
+    with on_device(x.device):
         prepared.wait()
         if training:
             y = _FP8Linear.apply(rows, weight, prepared)
         else:
-            y = fp8_matmul(quantize_fp8(rows.detach()), prepared.weight, dtype=x.dtype)
-    return y.view(*x.shape[:-1], weight.shape[0])
+            y = fp8_matmul(quantize_fp8(rows), prepared.weight, dtype=x.dtype)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], weight.shape[0])

@@ -14,12 +14,13 @@ together with its forward pass (autograd runs a backward pass on the stream of i
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._launch import on_device, stream_of
 
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 _SCORES = {"softmax": 0, "sigmoid": 1}
@@ -69,15 +70,6 @@ def _require_device(tensor, what):
         raise ValueError(f"{what} must be on a CUDA device")
 
 
-def _stream(*tensors):
-    """The current stream; it keeps the storage of tensors that were made on another one."""
-    stream = torch.cuda.current_stream()
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
-    return stream.cuda_stream
-
-
 def _rows(logits):
     """The logits as rows of unit column stride (copied only if they are not)."""
     tokens, experts = logits.shape
@@ -94,41 +86,65 @@ def _describe(logits, top_k, score, renormalize, scale, bias, padding_mask, sequ
         None if sequences is None else sequences.data_ptr())
 
 
-def _loss_buffers(router, device):
-    """(loss, table, workspace) of a call that computes the loss."""
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(tokens, experts, num_sequences):
+    router = _lib.WmRouter(logits=16, row_stride=experts, dtype=1, tokens=tokens, experts=experts,
+                           num_sequences=num_sequences, sequences=16 if num_sequences else None)
     size = ctypes.c_int64()
     _lib.check(_lib.load().wm_router_workspace(ctypes.byref(router), ctypes.byref(size)))
-    return (torch.empty((), dtype=torch.float32, device=device),
-            torch.empty(max(1, router.num_sequences) * router.experts + 1, dtype=torch.float32, device=device),
-            torch.empty(size.value, dtype=torch.uint8, device=device))
+    return size.value
+
+
+def _loss_buffers(logits, router):
+    """(loss, table, workspace) of a call that computes the loss."""
+    sequences = router.num_sequences
+    return (logits.new_empty((), dtype=torch.float32),
+            logits.new_empty(max(1, sequences) * router.experts + 1, dtype=torch.float32),
+            logits.new_empty(_workspace_bytes(router.tokens, router.experts, sequences), dtype=torch.uint8))
+
+
+def _address(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def _plain_gradient(gradient):
+    """An incoming gradient as contiguous FP32 (broadcast ones are expanded)."""
+    if gradient is None or (gradient.dtype == torch.float32 and gradient.is_contiguous()):
+        return gradient
+    return gradient.float().contiguous()
 
 
 def _backward(logits, router_args, routes, dgates, table, dloss):
-    with torch.cuda.device(logits.device):
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if torch.is_grad_enabled():
+        raise RuntimeError("The router's gradients cannot be differentiated again")
+    dgates, dloss = _plain_gradient(dgates), _plain_gradient(dloss)
+    device = logits.device
+    with on_device(device):
+        dlogits = logits.new_empty(logits.shape)
         router = _describe(logits, *router_args)
         _lib.check(_lib.load().wm_router_backward(
-            ctypes.byref(router), _lib.ptr(routes), _lib.ptr(dgates), _lib.ptr(table), _lib.ptr(dloss),
-            _lib.ptr(dlogits), _stream(logits, *router_args[-2:], routes, dgates, table, dloss)))
+            ctypes.byref(router), _address(routes), _address(dgates), _address(table), _address(dloss),
+            dlogits.data_ptr(), stream_of(device, logits, *router_args[-2:], routes, dgates, table, dloss)))
     return dlogits
 
 
 def _route(logits, top_k, score, renormalize, scale, bias, padding_mask, sequences, balance):
     """(routes, gates, counts, loss, table); the last three are None without the loss."""
     device = logits.device
-    with torch.cuda.device(device):
-        routes = torch.empty((logits.shape[0], top_k), dtype=torch.int32, device=device)
-        gates = torch.empty((logits.shape[0], top_k), dtype=torch.float32, device=device)
+    tokens, experts = logits.shape
+    with on_device(device):
+        routes = logits.new_empty((tokens, top_k), dtype=torch.int32)
+        gates = logits.new_empty((tokens, top_k), dtype=torch.float32)
         router = _describe(logits, top_k, score, renormalize, scale, bias, padding_mask, sequences)
         counts = loss = table = workspace = None
         if balance:
-            loss, table, workspace = _loss_buffers(router, device)
-            shape = (logits.shape[1],) if sequences is None else (sequences.shape[0] - 1, logits.shape[1])
-            counts = torch.empty(shape, dtype=torch.int32, device=device)
+            loss, table, workspace = _loss_buffers(logits, router)
+            counts = logits.new_empty((experts,) if sequences is None else (router.num_sequences, experts),
+                                      dtype=torch.int32)
         _lib.check(_lib.load().wm_router_forward(
-            ctypes.byref(router), _lib.ptr(routes), _lib.ptr(gates), _lib.ptr(counts), _lib.ptr(loss),
-            _lib.ptr(table), _lib.ptr(workspace), 0 if workspace is None else workspace.numel(),
-            _stream(logits, bias, padding_mask, sequences)))
+            ctypes.byref(router), routes.data_ptr(), gates.data_ptr(), _address(counts), _address(loss),
+            _address(table), _address(workspace), 0 if workspace is None else workspace.numel(),
+            stream_of(device, logits, bias, padding_mask, sequences)))
     return routes, gates, counts, loss, table
 
 
@@ -140,14 +156,16 @@ class _Route(torch.autograd.Function):
         ctx.options = (top_k, score, renormalize, scale)
         ctx.save_for_backward(rows, routes, padding_mask)
         ctx.mark_non_differentiable(routes)
+        ctx.set_materialize_grads(False)   # no zeros for the routes
         return routes, gates
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _, dgates):
+        if dgates is None:
+            return (None,) * 7
         rows, routes, padding_mask = ctx.saved_tensors
         dlogits = _backward(rows, (*ctx.options, None, padding_mask, None), routes,
-                            dgates.float().contiguous(), None, None)
+                            dgates, None, None)
         return (dlogits, *[None] * 6)
 
 
@@ -164,19 +182,14 @@ class _RouteAndBalance(torch.autograd.Function):
         return routes, gates, counts, loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _routes, dgates, _counts, dloss):
         rows, routes, padding_mask, sequences, table = ctx.saved_tensors
         if dgates is None and dloss is None:
             return (None,) * 8
         if dgates is None:
             routes = None
-        else:
-            dgates = dgates.float().contiguous()
         if dloss is None:
             table = None
-        else:
-            dloss = dloss.float().contiguous()
         dlogits = _backward(rows, (*ctx.options, None, padding_mask, sequences), routes, dgates, table, dloss)
         return (dlogits, *[None] * 7)
 
@@ -191,21 +204,21 @@ class _Balance(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
         rows, padding_mask, sequences, table = ctx.saved_tensors
         dlogits = _backward(rows, (1, ctx.score, False, 1.0, None, padding_mask, sequences), None, None, table,
-                            dloss.float().contiguous())
+                            dloss)
         return (dlogits, *[None] * 4)
 
 
 def _balance(rows, counts, score, padding_mask, sequences):
-    with torch.cuda.device(rows.device):
+    device = rows.device
+    with on_device(device):
         router = _describe(rows, 1, score, False, 1.0, None, padding_mask, sequences)
-        loss, table, workspace = _loss_buffers(router, rows.device)
+        loss, table, workspace = _loss_buffers(rows, router)
         _lib.check(_lib.load().wm_balance_forward(
-            ctypes.byref(router), _lib.ptr(counts), _lib.ptr(loss), _lib.ptr(table), _lib.ptr(workspace),
-            workspace.numel(), _stream(rows, counts, padding_mask, sequences)))
+            ctypes.byref(router), counts.data_ptr(), loss.data_ptr(), table.data_ptr(), workspace.data_ptr(),
+            workspace.numel(), stream_of(device, rows, counts, padding_mask, sequences)))
     return loss, table
 
 
@@ -244,13 +257,13 @@ def expert_counts(routes, experts, *, sequences=None):
         raise ValueError(f"experts must be in [1, {MAX_EXPERTS}]")
     _check_sequences(sequences, routes)
     _require_device(routes, "routes")
-    with torch.cuda.device(routes.device):
-        shape = (experts,) if sequences is None else (sequences.shape[0] - 1, experts)
-        counts = torch.empty(shape, dtype=torch.int32, device=routes.device)
+    device = routes.device
+    with on_device(device):
+        counts = routes.new_empty((experts,) if sequences is None else (sequences.shape[0] - 1, experts))
         _lib.check(_lib.load().wm_expert_counts(
-            _lib.ptr(routes), routes.shape[0], routes.shape[1], experts, _lib.ptr(sequences),
-            0 if sequences is None else sequences.shape[0] - 1, _lib.ptr(counts),
-            _stream(routes, sequences)))
+            routes.data_ptr(), routes.shape[0], routes.shape[1], experts, _address(sequences),
+            0 if sequences is None else sequences.shape[0] - 1, counts.data_ptr(),
+            stream_of(device, routes, sequences)))
     return counts
 
 
