@@ -7,7 +7,8 @@ S the sum of the terms' magnitudes: a block's 128 products are exact, their FP32
 import pytest
 import torch
 
-from weftmoe_b200.fp8 import (FP8Tensor, fp8_linear, fp8_matmul, poll_fp8_matmul, prepare_fp8_linear, quantize_fp8)
+from weftmoe_b200.fp8 import (FP8Tensor, _quantize_fp8_both, fp8_linear, fp8_matmul, poll_fp8_matmul,
+                              prepare_fp8_linear, quantize_fp8)
 
 pytestmark = pytest.mark.gpu
 
@@ -185,6 +186,33 @@ def test_offsets_beyond_32_bits():
     got = fp8_matmul(a, b)
     assert torch.equal(got[-5:], (wide(a)[-5:] @ wide(b).t()).float().bfloat16())
     assert torch.equal(got[:5], (wide(a)[:5] @ wide(b).t()).float().bfloat16())
+
+
+# ------------------------------------------------------------------ quantising both ways
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("rows, cols", [(1, 8), (1, 1), (127, 128), (128, 136), (129, 264), (300, 77), (1000, 520)])
+def test_both_ways_at_once_are_the_two_ways(rows, cols, dtype):
+    x = torch.randn(rows, cols, device="cuda", generator=generator(30)).to(dtype)
+    x[0, 0], x[rows // 2, cols // 2] = 3e38, 0.0
+    x[:, cols // 3] = 0.0
+    if rows > 100:
+        x[100, 3], x[rows - 1, cols - 1] = float("nan"), float("inf")
+    for source in (x, torch.cat([x, x])[rows:], x.new_empty(rows * cols + 1)[1:].view(rows, cols).copy_(x)):
+        straight, flipped = _quantize_fp8_both(source)
+        # the plain definition on both: by way of the FP32 source, whose kernel is another one
+        for got, want in ((straight, quantize_fp8(x.float())), (flipped, quantize_fp8(x.float(), transpose=True)),
+                          (flipped, quantize_fp8(source, transpose=True))):
+            assert got.shape == want.shape and got.block_rows == want.block_rows == 1
+            assert torch.equal(got.data.view(torch.uint8), want.data.view(torch.uint8))
+            assert torch.equal(got.scales.view(torch.int32), want.scales.view(torch.int32))
+
+
+def test_both_ways_of_several_matrices():
+    x = torch.randn(3, 200, 256, device="cuda", generator=generator(31)).bfloat16()
+    straight, flipped = _quantize_fp8_both(x)
+    for e in range(3):
+        assert torch.equal(straight.matrix(e).dequantize(), quantize_fp8(x[e]).dequantize())
+        assert torch.equal(flipped.matrix(e).dequantize(), quantize_fp8(x[e], transpose=True).dequantize())
 
 
 # ------------------------------------------------------------------ the projection

@@ -74,6 +74,7 @@ SIGNATURES = {
     "wm_runtime_read_timing": (c_int, [c_void_p, POINTER(ctypes.c_double), POINTER(ctypes.c_longlong), c_int]),
     "wm_route_plan": (c_int, [c_int32] * 8 + [c_void_p, c_void_p, POINTER(WmRouteOut), c_void_p]),
     "wm_fp8_quantize": (c_int, [c_void_p] + [c_int32] * 6 + [c_void_p, c_void_p, c_void_p]),
+    "wm_fp8_quantize_both": (c_int, [c_void_p] + [c_int32] * 4 + [c_void_p] * 5),
     "wm_fp8_quantize_weight": (c_int, [c_void_p] + [c_int32] * 4 + [c_void_p] * 5),
     "wm_fp8_transpose_weight": (c_int, [c_void_p, c_void_p] + [c_int32] * 3 + [c_void_p] * 3),
     "wm_fp8_gemm": (c_int, [c_void_p] * 5 + [c_int32] * 7 + [c_void_p]),

@@ -119,6 +119,18 @@ def quantize_fp8(tensor: torch.Tensor, *, block_rows: int = 1, transpose: bool =
     return out
 
 
+def _quantize_fp8_both(tensor: torch.Tensor) -> tuple[FP8Tensor, FP8Tensor]:
+    """1 x 128 blocks of a matrix and of its transpose from one pass over it: what `quantize_fp8` gives for either."""
+    _require_cuda(tensor, _SOURCE_DTYPES, "quantize_fp8")
+    with on_device(tensor.device):
+        straight = _allocate(tuple(tensor.shape), 1, tensor)
+        flipped = _allocate(_swap_last_two(tuple(tensor.shape)), 1, tensor)
+        _lib.check(_lib.load().wm_fp8_quantize_both(
+            *_source_args(tensor), straight.data.data_ptr(), straight.scales.data_ptr(), flipped.data.data_ptr(),
+            flipped.scales.data_ptr(), stream_of(tensor.device, tensor)))
+    return straight, flipped
+
+
 def _quantize_fp8_weight_pair(tensor: torch.Tensor) -> tuple[FP8Tensor, FP8Tensor]:
     """W and W^T with 128 x 128 blocks from one pass over the source: both orientations hold the same
     bytes and the same block scales (reference kernel: src/cuda/fp8/quantization.cuh:157-237)."""
@@ -417,23 +429,35 @@ def prepare_fp8_linear(weight, *, training: bool = True) -> PreparedFP8Linear:
 class _FP8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, prepared):
-        ctx.prepared = prepared
-        ctx.save_for_backward(x, weight)   # the weight: detects optimizer updates before backward
-        return fp8_matmul(quantize_fp8(x), prepared.weight, dtype=x.dtype)
+        ctx.prepared, ctx.x_type = prepared, x.dtype
+        held = ()
+        if ctx.needs_input_grad[1]:             # kept for dW instead of x: the blocks along the tokens, a byte each
+            rows, columns = _quantize_fp8_both(x)
+            held = (columns.data, columns.scales)
+            ctx.columns_shape = columns.shape
+        else:
+            rows = quantize_fp8(x)
+        ctx.save_for_backward(weight, *held)    # the weight: detects optimizer updates before backward
+        return fp8_matmul(rows, prepared.weight, dtype=x.dtype)
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():
             raise RuntimeError("The gradients of fp8_linear cannot be differentiated again")
-        x, weight = ctx.saved_tensors
-        prepared = ctx.prepared
-        dx = dweight = None
+        weight, *held = ctx.saved_tensors
+        to_x, to_weight, _ = ctx.needs_input_grad
         dy = dy.contiguous()
-        if ctx.needs_input_grad[0]:
-            dx = fp8_matmul(quantize_fp8(dy), prepared.weight_t, dtype=x.dtype)
-        if ctx.needs_input_grad[1]:
-            dweight = fp8_matmul(quantize_fp8(dy, transpose=True), quantize_fp8(x, transpose=True),
-                                 dtype=weight.dtype)
+        dx = dweight = rows = columns = None
+        if to_x and to_weight:
+            rows, columns = _quantize_fp8_both(dy)
+        elif to_x:
+            rows = quantize_fp8(dy)
+        else:
+            columns = quantize_fp8(dy, transpose=True)
+        if to_x:
+            dx = fp8_matmul(rows, ctx.prepared.weight_t, dtype=ctx.x_type)
+        if to_weight:
+            dweight = fp8_matmul(columns, FP8Tensor(*held, ctx.columns_shape), dtype=weight.dtype)
         return dx, dweight, None
 
 
