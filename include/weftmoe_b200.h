@@ -244,12 +244,18 @@ WM_API int wm_fp8_gemm(const void* aq, const float* as, const void* bq, const fl
  * captured.  aq / bq: E4M3 bytes, rows ceil128(k) apart (bytes behind k are not read), 16-byte aligned; as / bs: FP32
  * scales [ceil(rows / block_rows)][ceil(k / 128)], block rows 1 or 128, any values: each block of 128 along K is
  * summed in FP32 on the tensor cores and added times the product of its two scales in FP32.
+ * workspace (optional, NULL = none; wm_fp8_matmul_workspace bytes of device memory, 128-byte aligned, free again when
+ * the call's kernels are done): large products whose scales are all powers of two are then scaled on the tensor cores and
+ * summed there over up to 32 blocks, which is faster; the scales are looked at on the device.
  * out: rows ld >= n elements apart, BF16 (rounded once) or FP32; accumulate adds into an FP32 out.  k == 0 gives zeros.
  * wm_fp8_matmul_status synchronises `stream`, reads and clears the device's word: *code = WM_ERR_TIMEOUT when a
  * bounded wait of an earlier call ran out (that call's out is then incomplete). */
 WM_API int wm_fp8_matmul(const void* aq, const float* as, const void* bq, const float* bs, void* out, int64_t ld,
                          int32_t m, int32_t n, int32_t k, int32_t a_block_rows, int32_t b_block_rows,
-                         int32_t out_is_f32, int32_t accumulate, void* stream);
+                         int32_t out_is_f32, int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+/* Bytes of the workspace a product of these sizes can use on the current device; 0 where it uses none. */
+WM_API int wm_fp8_matmul_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes);
 WM_API int wm_fp8_matmul_status(int32_t* code, void* stream);
 
 /* ------------------------------------------------------------------------------------------

@@ -7,7 +7,8 @@ import torch
 from weftmoe_b200 import _lib
 from weftmoe_b200.fp8 import fp8_linear, fp8_matmul, prepare_fp8_linear
 
-GOOD = dict(aq=256, a_s=64, bq=256, bs=64, out=64, ld=16, m=8, n=16, k=128, a_rows=1, b_rows=128, f32=0, acc=0)
+GOOD = dict(aq=256, a_s=64, bq=256, bs=64, out=64, ld=16, m=8, n=16, k=128, a_rows=1, b_rows=128, f32=0, acc=0,
+            room=None, room_bytes=0)
 
 
 @pytest.mark.parametrize("change", [

@@ -78,7 +78,8 @@ SIGNATURES = {
     "wm_fp8_quantize_weight": (c_int, [c_void_p] + [c_int32] * 4 + [c_void_p] * 5),
     "wm_fp8_transpose_weight": (c_int, [c_void_p, c_void_p] + [c_int32] * 3 + [c_void_p] * 3),
     "wm_fp8_gemm": (c_int, [c_void_p] * 5 + [c_int32] * 7 + [c_void_p]),
-    "wm_fp8_matmul": (c_int, [c_void_p] * 5 + [c_int64] + [c_int32] * 7 + [c_void_p]),
+    "wm_fp8_matmul": (c_int, [c_void_p] * 5 + [c_int64] + [c_int32] * 7 + [c_void_p, c_int64, c_void_p]),
+    "wm_fp8_matmul_workspace": (c_int, [c_int32] * 3 + [POINTER(c_int64)]),
     "wm_fp8_matmul_status": (c_int, [POINTER(c_int32), c_void_p]),
     "wm_nvfp4_quantize": (c_int, [c_void_p, c_int32, c_int32, c_float, c_void_p, c_void_p, c_int32, c_void_p]),
     "wm_nvfp4_gemm": (c_int, [c_void_p] * 5 + [c_int32] * 3 + [c_float, c_int32, c_void_p]),

@@ -16,6 +16,11 @@
 // barrier, one commit per block, both frees the stage and hands its accumulator to the adding warps.
 // PAIR: two CTAs compute one 256 x 256 tile with cta_group::2, each fetching its own 128 rows of P and half of Q's 256,
 // so a byte of either operand feeds twice the arithmetic of a 128 x 128 tile.
+// PAIR, scales all powers of two (what this library's quantisers give): the tensor cores apply the scales themselves
+// (kind::mxf8f6f4.block_scale, scales as UE8M0 in TMEM) and accumulate up to 32 blocks before the adding warps take them
+// over.  The accumulator cuts what it cannot hold, so its error grows with the number of blocks (4.9e-7 of the result at
+// K = 8192, 3.0e-6 at 32768, against 1.3e-7 of FP32 sums of products); 32 blocks keep it below 3e-7.  A kernel in front packs the
+// scales and notes whether one is no power of two; the product then takes the general form above.
 // Otherwise `split` CTAs of a cluster may share one tile, each a range of the blocks; their sums are joined through
 // distributed shared memory in a fixed order.
 #include "../../include/weftmoe_b200.h"
@@ -29,6 +34,8 @@ namespace {
 __device__ int g_matmul_status;   // a bounded wait that ran out (read by wm_fp8_matmul_status)
 
 constexpr int kScaleChunk = 8;    // blocks of scales held at a time
+constexpr int kGroupBlocks = 32;  // blocks that the tensor cores accumulate when they apply the scales
+constexpr int kPackBlocks = 32;   // blocks of K that one CTA of the packing kernel takes
 
 struct MatmulArgs {
   const float* p_scales;
@@ -42,6 +49,8 @@ struct MatmulArgs {
   int out_is_f32, accumulate;
   int vector_store;               // rows of out are 16-byte aligned
   int tma_store;                  // ... and tmap_out describes them
+  const int* findings;            // of the packing kernel: non-zero where a scale is no power of two; null = not packed
+  int num_findings;
 };
 
 // ---------------------------------------------------------------- instructions
@@ -137,6 +146,22 @@ __device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
 __device__ __forceinline__ void arrive_in_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// Block-scaled MMA on a CTA pair (one UE8M0 scale per row and 32 elements of K, in TMEM), and the copy that brings a
+// 512-byte chunk of scales from each CTA's shared memory to its TMEM.
+__device__ __forceinline__ void umma_mxf8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                               uint32_t accumulate, uint32_t tmem_sfa, uint32_t tmem_sfb) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_cp_pair(uint32_t taddr, uint64_t smem_desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");
+}
 template <int REGS>
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 template <int REGS>
@@ -154,19 +179,25 @@ struct Matmul {
   static constexpr int kStageBytes = kPBytes + kQBytes;
   static constexpr int kBuffers = BN == 256 ? 2 : 4;             // accumulators in TMEM
   static constexpr int kColumns = BN * kBuffers < 32 ? 32 : BN * kBuffers;
-  static constexpr int kStages = PAIR ? 4 : BN == 128 ? 5 : 8;
+  static constexpr int kStages = PAIR ? 5 : BN == 128 ? 5 : 8;
   static_assert(kStages >= kBuffers, "an adding warp is never a whole round of stages behind the MMA");
   // Scales: [2][kScaleChunk][pitch] of P, then of Q.  Eight lanes copy the eight blocks of one row (one 32-byte
   // sector); the pitch of 4 (mod 32) words keeps those eight and the next three rows in different banks.
   static constexpr int kPitchP = 128 + 4;
   static constexpr int kPitchQ = Q_COLS ? BN + 4 : 4;
   static constexpr int kScaleBytes = 2 * kScaleChunk * (kPitchP + kPitchQ) * 4;
-  static constexpr int kStoreBytes = SWAP ? 0 : kCols * 32 * 2;  // staging of one adding warp
+  static constexpr int kStoreBytes = SWAP ? 0 : 4096;            // staging of one adding warp: a box of 32 rows x 128 bytes
   static constexpr int kScalesAt = kStages * kStageBytes + EPI * kStoreBytes;
   static constexpr int kBarriersAt = kScalesAt + kScaleBytes;
   static constexpr int kTotal = kBarriersAt + 256 + 1024;
   static_assert(kScalesAt % 16 == 0 && kTotal <= 227 * 1024, "shared memory");
   static_assert(PAIR || BN * 128 * 4 <= kStages * kStageBytes, "the joined sums fit in the stages");
+  // PAIR with packed scales: chunks of 128 rows' scales of four blocks, one of P and two of Q, come with every fourth
+  // stage, in place of the table; in TMEM twice behind the one accumulator, 16 columns each.  (A chunk for every block, the
+  // same byte four times, took 131 us for 8192 x 4096 x 4096 where four blocks a chunk take 117.)
+  static constexpr int kPackedBytes = 3 * 512;
+  static constexpr uint32_t kTmemScales = BN;
+  static_assert(!PAIR || kStages * kPackedBytes <= kScaleBytes, "packed scales fit where the table is");
   // PAIR: the four service warps give registers to the eight adding warps: 128 x 56 + 256 x 224 = 384 x 168, what
   // the block is launched with (checked before the first launch).
   static constexpr int kRegisters = 168, kLow = 56, kHigh = 224;
@@ -229,40 +260,33 @@ __device__ __forceinline__ void store_row(const MatmulArgs& a, int p, int q, con
 template <int PAIRS>
 __device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorMap* tmap, uint8_t* staging, int p, int q,
                                             int lane, const uint64_t (&sum)[PAIRS]) {
-  constexpr int kBoxes = PAIRS / 32;                     // boxes that fit in the staging at once
-  const int passes = a.out_is_f32 ? 2 : 1;
+  uint8_t* line = staging + lane * 128;
+  const int boxes = a.out_is_f32 ? PAIRS / 16 : PAIRS / 32;
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    if (pass == passes) break;
-    if (lane == 0) bulk_wait_group_read<0>();            // the boxes before these have left the staging
+  for (int b = 0; b < PAIRS / 16; ++b) {
+    if (b == boxes) break;
+    if (lane == 0) bulk_wait_group_read<0>();            // the box before this one has left the staging
     __syncwarp();
 #pragma unroll
-    for (int b = 0; b < kBoxes; ++b) {
-      uint8_t* line = staging + b * 4096 + lane * 128;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 w;
-        if (a.out_is_f32) {
-          const int from = ((pass * kBoxes + b) * 32 + c * 4) / 2;
-          const float2 x = halves_of(sum[from]), y = halves_of(sum[from + 1]);
-          w = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
-        } else {
-          const int from = (b * 64 + c * 8) / 2;
-          const float2 x = halves_of(sum[from]), y = halves_of(sum[from + 1]), z = halves_of(sum[from + 2]),
-                       t = halves_of(sum[from + 3]);
-          w = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(y.x, y.y), pack_bf16x2(z.x, z.y), pack_bf16x2(t.x, t.y));
-        }
-        *reinterpret_cast<uint4*>(line + ((c ^ (lane & 7)) << 4)) = w;
+    for (int c = 0; c < 8; ++c) {
+      uint4 w;
+      if (a.out_is_f32) {
+        const int from = b * 16 + c * 2;
+        const float2 x = halves_of(sum[from]), y = halves_of(sum[from + 1]);
+        w = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
+      } else {
+        const int from = (b * 32 + c * 4) % PAIRS;       // (boxes behind the last are not reached)
+        const float2 x = halves_of(sum[from]), y = halves_of(sum[from + 1]), z = halves_of(sum[from + 2]),
+                     t = halves_of(sum[from + 3]);
+        w = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(y.x, y.y), pack_bf16x2(z.x, z.y), pack_bf16x2(t.x, t.y));
       }
+      *reinterpret_cast<uint4*>(line + ((c ^ (lane & 7)) << 4)) = w;
     }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-#pragma unroll
-      for (int b = 0; b < kBoxes; ++b) {
-        const int x = q + (a.out_is_f32 ? (pass * kBoxes + b) * 32 : b * 64);
-        if (p < a.p_rows && x < a.q_rows) tma_store_2d(tmap, staging + b * 4096, x, p);
-      }
+      const int x = q + b * (a.out_is_f32 ? 32 : 64);
+      if (p < a.p_rows && x < a.q_rows) tma_store_2d(tmap, staging, x, p);
       bulk_commit_group();
     }
   }
@@ -272,7 +296,8 @@ __device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorM
 template <int BN, int EPI, bool SWAP, bool Q_COLS, bool PAIR>
 __global__ void __launch_bounds__(128 + 32 * EPI, 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
-                  const __grid_constant__ CUtensorMap tmap_out, const MatmulArgs a) {
+                  const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_sp,
+                  const __grid_constant__ CUtensorMap tmap_sq, const MatmulArgs a) {
   using S = Matmul<BN, EPI, SWAP, Q_COLS, PAIR>;
   constexpr int kCols = S::kCols, kLoad = S::kLoad;
   extern __shared__ uint8_t smem_raw[];
@@ -285,7 +310,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   uint64_t* tmem_empty = done_bar + S::kStages;                              // the leader's
   uint64_t* scale_full = tmem_empty + S::kBuffers;
   uint64_t* scale_empty = scale_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(scale_empty + 2);
+  uint64_t* group_full = scale_empty + 2;                                    // packed scales: accumulator ready, in both
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(group_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = PAIR ? static_cast<int>(cluster_ctarank()) : 0;            // 0 = leader
@@ -301,6 +327,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
       mbar_init(scale_full + s, 64);
       mbar_init(scale_empty + s, EPI);
     }
+    mbar_init(group_full, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_p);
@@ -315,6 +342,16 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   if constexpr (PAIR) cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+
+  bool packed = false;
+  if constexpr (PAIR) {
+    cudaGridDependencySynchronize();   // launched while the packing kernel still runs
+    if (a.findings != nullptr) {
+      int found = 0;
+      for (int i = threadIdx.x; i < a.num_findings; i += S::kThreads) found |= __ldcg(a.findings + i);
+      packed = __syncthreads_or(found) == 0;
+    }
+  }
 
   const int group = PAIR ? 2 : a.split;    // CTAs of a tile
   const int kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * part / a.split);
@@ -337,9 +374,17 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
           uint8_t* sp = smem + stage * S::kStageBytes;
           if constexpr (PAIR) {
             const uint32_t bar = map_to_cta(smem_u32(full_bar + stage), 0);
-            if (cta == 0) mbar_expect_tx(full_bar + stage, 2 * S::kStageBytes);
+            const bool scales_too = packed && kb % 4 == 0;
+            if (cta == 0) mbar_expect_tx(full_bar + stage, 2 * (S::kStageBytes + (scales_too ? S::kPackedBytes : 0)));
             tma_load_2d_pair(sp, &tmap_p, bar, kb * 128, t.p0 + cta * 128);
             tma_load_2d_pair(sp + S::kPBytes, &tmap_q, bar, kb * 128, t.q0 + cta * (BN / 2));
+            if (scales_too) {   // a chunk is four rows of 128 bytes; each CTA holds the scales of all 256 columns
+              uint8_t* sf = smem + S::kScalesAt + stage * S::kPackedBytes;
+              const int chunks = (a.kblocks + 3) / 4;
+              tma_load_2d_pair(sf, &tmap_sp, bar, 0, ((t.p0 >> 7) + cta) * chunks * 4 + kb);
+              tma_load_2d_pair(sf + 512, &tmap_sq, bar, 0, (t.q0 >> 7) * chunks * 4 + kb);
+              tma_load_2d_pair(sf + 1024, &tmap_sq, bar, 0, ((t.q0 >> 7) + 1) * chunks * 4 + kb);
+            }
           } else {
             mbar_expect_tx(full_bar + stage, S::kStageBytes);
             tma_load_2d(sp, &tmap_p, full_bar + stage, kb * 128, t.p0);
@@ -354,6 +399,39 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
+      if constexpr (PAIR) {
+        if (packed) {
+          for (int tile = first; ok && tile < tiles; tile += step) {
+            for (int kb = 0; kb < a.kblocks; ++kb) {
+              const bool opens = kb % kGroupBlocks == 0;
+              if (opens) {
+                ok = mbar_wait(tmem_empty, buffer_phase ^ 1, abort_flag, &g_matmul_status, kStatusTimeoutTmemEmpty);
+                buffer_phase ^= 1;
+              }
+              ok = ok && mbar_wait(full_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutSmemFull);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t sp = smem_u32(smem + stage * S::kStageBytes);
+              const uint64_t dp = umma_desc_sw128(sp, 0, 1024), dq = umma_desc_sw128(sp + S::kPBytes, 0, 1024);
+              const uint32_t sfp = tmem_base + S::kTmemScales + (kb / 4 % 2) * 16, sfq = sfp + 4;
+              if (kb % 4 == 0) {
+                const uint64_t sf = umma_desc_noswizzle(smem_u32(smem + S::kScalesAt + stage * S::kPackedBytes), 128);
+                tmem_cp_pair(sfp, sf);
+                tmem_cp_pair(sfq, sf + 32);
+                tmem_cp_pair(sfq + 4, sf + 64);
+              }
+              const uint32_t idesc_kb = umma_idesc_block_scaled(0u, 1u, 256, BN, kb & 3, kb & 3);   // byte of the chunk
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_mxf8_pair(tmem_base, dp + 2 * k, dq + 2 * k, idesc_kb, opens && k == 0 ? 0u : 1u, sfp, sfq);
+              umma_commit_both(done_bar + stage);
+              if (kb + 1 == a.kblocks || (kb + 1) % kGroupBlocks == 0) umma_commit_both(group_full);
+              if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+            }
+          }
+          ok = false;   // the loop below is the other form's
+        }
+      }
       for (int tile = first; ok && tile < tiles; tile += step) {
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(tmem_empty + buffer, buffer_phase ^ 1, abort_flag, &g_matmul_status, kStatusTimeoutTmemEmpty) &&
@@ -373,7 +451,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
           if (++buffer == S::kBuffers) { buffer = 0; buffer_phase ^= 1; }
         }
       }
-    } else if (warp >= 2) {
+    } else if (warp >= 2 && !packed) {
       // ------------------------------------------------------------ scales
       const int kb = lane & 7, row = (threadIdx.x - 64) >> 3;
       int held = 0;
@@ -425,11 +503,37 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
       for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
       // Loads run ahead of the additions by kLoad columns, across blocks too.
       uint32_t v[2][kLoad];
-      ok = mbar_wait(done_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
-      if (!ok) break;
-      tc_fence_after();
-      tmem_ld_cols<kLoad>(from + buffer * BN, v[0]);
-      for (int kb = kb0; kb < kb1; ++kb) {
+      if (PAIR && packed) {
+        for (int kb = 0; kb < a.kblocks; kb += kGroupBlocks) {
+          ok = mbar_wait(group_full, phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
+          if (!ok) break;
+          phase ^= 1;
+          tc_fence_after();
+          tmem_ld_cols<kLoad>(from, v[0]);
+#pragma unroll
+          for (int c = 0; c < kCols / kLoad; ++c) {
+            tmem_ld_wait_for<kLoad>(v[c & 1]);
+            if (c + 1 < kCols / kLoad) {
+              tmem_ld_cols<kLoad>(from + (c + 1) * kLoad, v[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) arrive_in_cluster(map_to_cta(smem_u32(tmem_empty), 0));
+            }
+#pragma unroll
+            for (int j = 0; j < kLoad / 2; ++j) {
+              const float2 w = halves_of(sum[c * (kLoad / 2) + j]);
+              sum[c * (kLoad / 2) + j] = pair_of(w.x + __uint_as_float(v[c & 1][2 * j]), w.y + __uint_as_float(v[c & 1][2 * j + 1]));
+            }
+          }
+        }
+      } else {
+        ok = mbar_wait(done_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld_cols<kLoad>(from + buffer * BN, v[0]);
+      }
+      for (int kb = PAIR && packed ? kb1 : kb0; kb < kb1; ++kb) {
         const int in_chunk = (kb - kb0) & (kScaleChunk - 1);
         if (in_chunk == 0) {
           ok = mbar_wait(scale_full + held, held_phase, abort_flag, &g_matmul_status, kStatusTimeoutTmemFull);
@@ -541,9 +645,76 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   }
 }
 
+// FP32 scales -> UE8M0 chunks [ceil(rows / 128)][ceil(kblocks / 4)][512 bytes] in the 4 x 32 order of tcgen05.cp (word
+// (r % 32) * 4 + r / 32 holds row r, byte i the block 4 c + i), of P and then of Q.  Rows and blocks behind the last get scale 1.  Each CTA, one of 128 rows x 32 blocks, notes whether it met a scale that is no power of two.
+__global__ void __launch_bounds__(256)
+pack_scales_kernel(const float* __restrict__ p_scales, int p_rows, int p_shift, uint32_t* __restrict__ p_out,
+                   const float* __restrict__ q_scales, int q_rows, int q_shift, uint32_t* __restrict__ q_out, int kblocks,
+                   int* __restrict__ findings) {
+  __shared__ unsigned char codes[kPackBlocks][128 + 4];
+  cudaTriggerProgrammaticLaunchCompletion();   // the product may take its place; it waits for these before it reads
+  const int p_tiles = (p_rows + 127) / 128;
+  const bool of_p = static_cast<int>(blockIdx.x) < p_tiles;
+  const int tile = of_p ? blockIdx.x : blockIdx.x - p_tiles;
+  const float* scales = of_p ? p_scales : q_scales;
+  const int rows = of_p ? p_rows : q_rows, shift = of_p ? p_shift : q_shift;
+  const int kb0 = blockIdx.y * kPackBlocks, count = min(kPackBlocks, kblocks - kb0);
+  int found = 0;
+  for (int i = threadIdx.x; i < 128 * kPackBlocks; i += 256) {
+    const int kb = i % kPackBlocks, r = i / kPackBlocks;
+    unsigned code = 127;
+    if (kb < count && tile * 128 + r < rows) {
+      const unsigned bits = __float_as_uint(__ldg(scales + static_cast<long long>((tile * 128 + r) >> shift) * kblocks + kb0 + kb));
+      code = bits >> 23;   // the biased exponent is the UE8M0 code
+      found |= (bits & 0x7fffffu) != 0 || code == 0 || code >= 255;   // mantissa, zero, infinite, negative
+    }
+    codes[kb][r] = static_cast<unsigned char>(code);
+  }
+  found = __syncthreads_or(found);
+  if (threadIdx.x == 0) findings[blockIdx.y * gridDim.x + blockIdx.x] = found;
+  const int chunks = (kblocks + 3) / 4, here = (count + 3) / 4;
+  uint32_t* out = (of_p ? p_out : q_out) + (static_cast<long long>(tile) * chunks + kb0 / 4) * 128;
+  for (int i = threadIdx.x; i < 128 * here; i += 256) {
+    const int c = i / 128 * 4, word = i % 128, r = (word >> 2) + 32 * (word & 3);
+    out[i] = codes[c][r] | codes[c + 1][r] << 8 | codes[c + 2][r] << 16 | static_cast<unsigned>(codes[c + 3][r]) << 24;
+  }
+}
+
+// What a product on CTA pairs with packed scales needs besides its operands.
+struct Packing {
+  int p_tiles, q_tiles, parts, chunks;
+  long long q_at, findings_at, bytes;
+};
+Packing packing_of(int m, int n, int kblocks) {
+  Packing k{};
+  k.p_tiles = (m + 127) / 128;
+  k.q_tiles = (n + 127) / 128;
+  k.parts = (kblocks + kPackBlocks - 1) / kPackBlocks;
+  k.chunks = (kblocks + 3) / 4;
+  k.q_at = static_cast<long long>(k.p_tiles) * k.chunks * 512;
+  k.findings_at = k.q_at + static_cast<long long>(k.q_tiles) * k.chunks * 512;
+  k.bytes = k.findings_at + static_cast<long long>(k.p_tiles + k.q_tiles) * k.parts * 4;
+  return k;
+}
+
+// Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  Pairs of SMs take 256 x 256 tiles where
+// those alone fill half of the pairs.
+bool takes_pairs(int m, int n, int sms) {
+  return m > 64 && static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * 4 >= sms;
+}
+// Packing costs a launch: where K is short the general form is done sooner.
+bool takes_packed(int m, int n, int kblocks, int sms) { return takes_pairs(m, n, sms) && kblocks >= 8; }
+
+int sm_count(int* sms) {
+  int dev = 0;
+  WM_CUDA(cudaGetDevice(&dev));
+  WM_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return WM_OK;
+}
+
 template <int BN, int EPI, bool SWAP, bool Q_COLS, bool PAIR>
-int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tout, MatmulArgs a, int sms,
-                  cudaStream_t stream) {
+int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tout, const CUtensorMap& tsp,
+                  const CUtensorMap& tsq, MatmulArgs a, int sms, cudaStream_t stream) {
   using S = Matmul<BN, EPI, SWAP, Q_COLS, PAIR>;
   auto kernel = fp8_matmul_kernel<BN, EPI, SWAP, Q_COLS, PAIR>;
   static PerDeviceOnce configured;  // one table per template instantiation
@@ -579,13 +750,15 @@ int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMa
   config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kTotal;
   config.stream = stream;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = group;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
-  WM_CUDA(cudaLaunchKernelEx(&config, kernel, tp, tq, tout, a));
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = group;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = PAIR && a.findings != nullptr ? 2 : 1;   // early only behind the packing kernel
+  WM_CUDA(cudaLaunchKernelEx(&config, kernel, tp, tq, tout, tsp, tsq, a));
   count_launch();
   return WM_OK;
 }
@@ -594,7 +767,8 @@ int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMa
 
 extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, const float* bs, void* out, int64_t ld,
                              int32_t m, int32_t n, int32_t k, int32_t a_block_rows, int32_t b_block_rows,
-                             int32_t out_is_f32, int32_t accumulate, void* stream_) {
+                             int32_t out_is_f32, int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                             void* stream_) {
   if (m < 0 || n < 0 || k < 0 || (a_block_rows != 1 && a_block_rows != 128) ||
       (b_block_rows != 1 && b_block_rows != 128) || ld < n || (accumulate && !out_is_f32)) {
     set_error("wm_fp8_matmul: [M,K] x [N,K], block rows 1 or 128, rows of out at least N apart; accumulation needs an "
@@ -620,14 +794,16 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   }
   const int kblocks = static_cast<int>((static_cast<long long>(k) + 127) / 128);
   const uint64_t pitch = static_cast<uint64_t>(kblocks) * 128;
-  int sms = 0, dev = 0;
-  WM_CUDA(cudaGetDevice(&dev));
-  WM_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  // Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  Pairs of SMs take 256 x 256 tiles
-  // where those alone fill half of the pairs.
-  const bool swap = m <= 64;
-  const bool pairs = !swap && static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * 4 >= sms;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const bool swap = m <= 64, pairs = takes_pairs(m, n, sms);
   const int bn = swap ? (m <= 16 ? 16 : m <= 32 ? 32 : 64) : 128;
+  const Packing packing = packing_of(m, n, kblocks);
+  const bool packed = workspace && takes_packed(m, n, kblocks, sms);
+  if (packed && (workspace_bytes < packing.bytes || reinterpret_cast<uintptr_t>(workspace) % 128)) {
+    set_error("wm_fp8_matmul: small or misaligned workspace (wm_fp8_matmul_workspace, 128-byte aligned)");
+    return WM_ERR_INVALID;
+  }
   MatmulArgs a{};
   a.p_scales = swap ? bs : as;
   a.q_scales = swap ? as : bs;
@@ -649,15 +825,43 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   a.tma_store = !swap && a.vector_store && !accumulate;
   if (a.tma_store)
     if (int rc = make_tmap_2d(&tout, out, element, n, m, static_cast<uint64_t>(ld) * element, 128 / element, 32)) return rc;
+  CUtensorMap tsp = tp, tsq = tp;   // not read without packed scales
+  if (packed) {
+    uint8_t* room = static_cast<uint8_t*>(workspace);
+    int* findings = reinterpret_cast<int*>(room + packing.findings_at);
+    pack_scales_kernel<<<dim3(packing.p_tiles + packing.q_tiles, packing.parts), 256, 0, stream>>>(
+        as, m, a.p_shift, reinterpret_cast<uint32_t*>(room), bs, n, a.q_shift,
+        reinterpret_cast<uint32_t*>(room + packing.q_at), kblocks, findings);
+    count_launch();
+    WM_CUDA(cudaGetLastError());
+    a.findings = findings;
+    a.num_findings = (packing.p_tiles + packing.q_tiles) * packing.parts;
+    const uint64_t rows_p = static_cast<uint64_t>(packing.p_tiles) * packing.chunks * 4;
+    const uint64_t rows_q = static_cast<uint64_t>(packing.q_tiles) * packing.chunks * 4;
+    if (int rc = make_tmap_2d(&tsp, room, 1, 128, rows_p, 128, 128, 4, false)) return rc;
+    if (int rc = make_tmap_2d(&tsq, room + packing.q_at, 1, 128, rows_q, 128, 128, 4, false)) return rc;
+  }
   const bool by_column = a.q_shift == 0;
-  if (bn == 16) return launch_matmul<16, 4, true, true, false>(tp, tq, tout, a, sms, stream);
-  if (bn == 32) return launch_matmul<32, 4, true, true, false>(tp, tq, tout, a, sms, stream);
-  if (bn == 64) return launch_matmul<64, 4, true, true, false>(tp, tq, tout, a, sms, stream);
+  if (bn == 16) return launch_matmul<16, 4, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
+  if (bn == 32) return launch_matmul<32, 4, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
+  if (bn == 64) return launch_matmul<64, 4, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
   if (pairs)
-    return by_column ? launch_matmul<256, 8, false, true, true>(tp, tq, tout, a, sms, stream)
-                     : launch_matmul<256, 8, false, false, true>(tp, tq, tout, a, sms, stream);
-  return by_column ? launch_matmul<128, 8, false, true, false>(tp, tq, tout, a, sms, stream)
-                   : launch_matmul<128, 8, false, false, false>(tp, tq, tout, a, sms, stream);
+    return by_column ? launch_matmul<256, 8, false, true, true>(tp, tq, tout, tsp, tsq, a, sms, stream)
+                     : launch_matmul<256, 8, false, false, true>(tp, tq, tout, tsp, tsq, a, sms, stream);
+  return by_column ? launch_matmul<128, 8, false, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream)
+                   : launch_matmul<128, 8, false, false, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
+}
+
+extern "C" int wm_fp8_matmul_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes) {
+  if (m < 0 || n < 0 || k < 0 || !bytes) {
+    set_error("wm_fp8_matmul_workspace: negative size or null result");
+    return WM_ERR_INVALID;
+  }
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const int kblocks = static_cast<int>((static_cast<long long>(k) + 127) / 128);
+  *bytes = takes_packed(m, n, kblocks, sms) ? packing_of(m, n, kblocks).bytes : 0;
+  return WM_OK;
 }
 
 extern "C" int wm_fp8_matmul_status(int32_t* code, void* stream_) {

@@ -56,9 +56,11 @@ struct TmapKey {
   uint64_t inner, outer, stride;
   uint32_t box_inner, box_outer;
   int elem_bytes;
+  bool swizzle;
   bool operator==(const TmapKey& o) const {
     return base == o.base && inner == o.inner && outer == o.outer && stride == o.stride &&
-           box_inner == o.box_inner && box_outer == o.box_outer && elem_bytes == o.elem_bytes;
+           box_inner == o.box_inner && box_outer == o.box_outer && elem_bytes == o.elem_bytes &&
+           swizzle == o.swizzle;
   }
 };
 struct TmapSlot {
@@ -70,12 +72,12 @@ constexpr int kTmapSlots = 256;  // direct-mapped; a collision just re-encodes
 }  // namespace
 
 static int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
-                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer);
+                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, bool swizzle);
 
 int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
-                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, bool swizzle) {
   static thread_local TmapSlot cache[kTmapSlots];
-  const TmapKey key{base, inner, outer, row_stride_bytes, box_inner, box_outer, elem_bytes};
+  const TmapKey key{base, inner, outer, row_stride_bytes, box_inner, box_outer, elem_bytes, swizzle};
   uint64_t h = reinterpret_cast<uintptr_t>(base) >> 4;
   h = (h ^ (inner * 0x9E3779B97F4A7C15ull) ^ (outer * 0xC2B2AE3D27D4EB4Full) ^ (box_outer * 0x165667B19E3779F9ull) ^
        (static_cast<uint64_t>(box_inner) << 7) ^ static_cast<uint64_t>(elem_bytes)) * 0xD6E8FEB86659FD93ull;
@@ -84,7 +86,8 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t in
     *out = slot.map;
     return 0;
   }
-  if (int rc = encode_tmap_2d(out, base, elem_bytes, inner, outer, row_stride_bytes, box_inner, box_outer)) return rc;
+  if (int rc = encode_tmap_2d(out, base, elem_bytes, inner, outer, row_stride_bytes, box_inner, box_outer, swizzle))
+    return rc;
   slot.key = key;
   slot.map = *out;
   slot.used = true;
@@ -92,7 +95,7 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t in
 }
 
 static int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
-                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, bool swizzle) {
   auto fn = encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
@@ -113,7 +116,7 @@ static int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, ui
                                                      : CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUresult r = fn(out, type,
                   2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d (inner %llu outer %llu)", (int)r,

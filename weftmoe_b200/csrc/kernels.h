@@ -50,9 +50,9 @@ inline int opt_in_dynamic_smem(Kernel kernel, int bytes, PerDeviceOnce& once) {
 
 // ------------------------------------------------------------------ tensor maps
 // 2-D BF16 (elem_bytes = 2) or 8-bit (elem_bytes = 1) row-major tensor, 128-byte swizzle.
-// box_inner * elem_bytes must be 128.  Returns 0 on success.
+// box_inner * elem_bytes must be 128.  swizzle = false leaves the box as it is.  Returns 0 on success.
 int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
-                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer);
+                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, bool swizzle = true);
 
 // ------------------------------------------------------------------ grouped GEMM launchers
 struct Schedule {

@@ -16,6 +16,7 @@ Storage rules:
 from __future__ import annotations
 
 import ctypes
+import functools
 import weakref
 from dataclasses import dataclass
 
@@ -190,6 +191,14 @@ def fp8_gemm(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Ten
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _matmul_workspace_bytes(m, n, k, device):
+    """Room that a product of these sizes uses (0: none); `device` is the current one, whose SMs it depends on."""
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().wm_fp8_matmul_workspace(m, n, k, ctypes.byref(size)))
+    return size.value
+
+
 def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Tensor | None = None,
                accumulate: bool = False) -> torch.Tensor:
     """A @ B^T of A [M, K] and B [N, K], blocks of 1 or 128 rows on either side, any scales.
@@ -214,10 +223,12 @@ def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.T
                     and out.device == device and (n <= 1 or out.stride(1) == 1) and (m <= 1 or out.stride(0) >= n))
             if not fits:
                 raise ValueError("FP8 output shape, dtype, device or layout mismatch")
+        size = _matmul_workspace_bytes(m, n, k, device.index)
+        workspace = a.scales.new_empty(size, dtype=torch.uint8) if size else None
         _lib.check(_lib.load().wm_fp8_matmul(
             a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(), out.data_ptr(),
             out.stride(0) if m > 1 else max(n, 1), m, n, k, a.block_rows, b.block_rows, int(dtype == torch.float32),
-            int(accumulate), stream_of(device, a.data, a.scales, b.data, b.scales)))
+            int(accumulate), None if workspace is None else workspace.data_ptr(), size, stream_of(device, a.data, a.scales, b.data, b.scales)))
     return out
 
 
