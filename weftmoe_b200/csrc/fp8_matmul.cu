@@ -393,9 +393,11 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
           if (++stage == S::kStages) { stage = 0; phase ^= 1; }
         }
       }
-    } else if (warp == 1 && lane == 0 && cta == 0) {
+    } else if (warp == 1 && cta == 0) {
       // ------------------------------------------------------------ MMA
-      constexpr uint32_t idesc = umma_idesc(0u, S::kRowsP, BN, 0u, 0u);
+      // The whole warp walks the blocks and one elected lane issues, so that descriptors and addresses stay in uniform
+      // registers: issued by a lane on its own, a block's four MMAs and commit took 462 cycles, more than the MMAs run.
+      const uint64_t d0 = umma_desc_sw128(smem_u32(smem), 0, 1024);
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
@@ -409,44 +411,52 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
                 buffer_phase ^= 1;
               }
               ok = ok && mbar_wait(full_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutSmemFull);
+              ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t sp = smem_u32(smem + stage * S::kStageBytes);
-              const uint64_t dp = umma_desc_sw128(sp, 0, 1024), dq = umma_desc_sw128(sp + S::kPBytes, 0, 1024);
+              const uint64_t dp = d0 + static_cast<uint32_t>(stage * (S::kStageBytes >> 4)), dq = dp + (S::kPBytes >> 4);
               const uint32_t sfp = tmem_base + S::kTmemScales + (kb / 4 % 2) * 16, sfq = sfp + 4;
-              if (kb % 4 == 0) {
-                const uint64_t sf = umma_desc_noswizzle(smem_u32(smem + S::kScalesAt + stage * S::kPackedBytes), 128);
-                tmem_cp_pair(sfp, sf);
-                tmem_cp_pair(sfq, sf + 32);
-                tmem_cp_pair(sfq + 4, sf + 64);
-              }
               const uint32_t idesc_kb = umma_idesc_block_scaled(0u, 1u, 256, BN, kb & 3, kb & 3);   // byte of the chunk
+              const bool closes = kb + 1 == a.kblocks || (kb + 1) % kGroupBlocks == 0;
+              if (elect_one()) {
+                if (kb % 4 == 0) {
+                  const uint64_t sf = umma_desc_noswizzle(smem_u32(smem + S::kScalesAt + stage * S::kPackedBytes), 128);
+                  tmem_cp_pair(sfp, sf);
+                  tmem_cp_pair(sfq, sf + 32);
+                  tmem_cp_pair(sfq + 4, sf + 64);
+                }
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_mxf8_pair(tmem_base, dp + 2 * k, dq + 2 * k, idesc_kb, opens && k == 0 ? 0u : 1u, sfp, sfq);
-              umma_commit_both(done_bar + stage);
-              if (kb + 1 == a.kblocks || (kb + 1) % kGroupBlocks == 0) umma_commit_both(group_full);
+                for (int k = 0; k < 4; ++k)
+                  umma_mxf8_pair(tmem_base, dp + 2 * k, dq + 2 * k, idesc_kb, opens && k == 0 ? 0u : 1u, sfp, sfq);
+                umma_commit_both(done_bar + stage);
+                if (closes) umma_commit_both(group_full);
+              }
+              __syncwarp();
               if (++stage == S::kStages) { stage = 0; phase ^= 1; }
             }
           }
           ok = false;   // the loop below is the other form's
         }
       }
+      constexpr uint32_t idesc = umma_idesc(0u, S::kRowsP, BN, 0u, 0u);
       for (int tile = first; ok && tile < tiles; tile += step) {
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(tmem_empty + buffer, buffer_phase ^ 1, abort_flag, &g_matmul_status, kStatusTimeoutTmemEmpty) &&
                mbar_wait(full_bar + stage, phase, abort_flag, &g_matmul_status, kStatusTimeoutSmemFull);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sp = smem_u32(smem + stage * S::kStageBytes);
-          const uint64_t dp = umma_desc_sw128(sp, 0, 1024), dq = umma_desc_sw128(sp + S::kPBytes, 0, 1024);
+          const uint64_t dp = d0 + static_cast<uint32_t>(stage * (S::kStageBytes >> 4)), dq = dp + (S::kPBytes >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (PAIR) umma_f8_pair(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
-            else umma_f8(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (PAIR) umma_f8_pair(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
+              else umma_f8(tmem_base + buffer * BN, dp + 2 * k, dq + 2 * k, idesc, k != 0 ? 1u : 0u);
+            }
+            if constexpr (PAIR) umma_commit_both(done_bar + stage);
+            else umma_commit(done_bar + stage);
           }
-          if constexpr (PAIR) umma_commit_both(done_bar + stage);
-          else umma_commit(done_bar + stage);
+          __syncwarp();
           if (++stage == S::kStages) { stage = 0; phase ^= 1; }
           if (++buffer == S::kBuffers) { buffer = 0; buffer_phase ^= 1; }
         }
