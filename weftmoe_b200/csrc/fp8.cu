@@ -135,6 +135,7 @@ __global__ void quantize_tile_kernel(const T* __restrict__ x, int rows, int cols
 // own one 1 x 128 block, eight consecutive values per lane (one 16-byte load, one 8-byte store).
 __global__ void quantize_rows_bf16_kernel(const uint4* __restrict__ x, long long blocks, int cblocks,
                                           uint2* __restrict__ q, float* __restrict__ s) {
+  cudaTriggerProgrammaticLaunchCompletion();   // a product behind this may set itself up; it waits before it reads
   const long long half_warps = (static_cast<long long>(gridDim.x) * blockDim.x) >> 4;
   const int sub = threadIdx.x & 15;
   const unsigned mask = 0xffffu << (threadIdx.x & 16);

@@ -343,9 +343,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
+  cudaGridDependencySynchronize();   // launched while the kernel before still runs: nothing is read or written until here
   bool packed = false;
   if constexpr (PAIR) {
-    cudaGridDependencySynchronize();   // launched while the packing kernel still runs
     if (a.findings != nullptr) {
       int found = 0;
       for (int i = threadIdx.x; i < a.num_findings; i += S::kThreads) found |= __ldcg(a.findings + i);
@@ -635,12 +635,30 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
       const Tile t = tile_at<S::kRowsP, BN>(a, first);
       const int row = (warp & 3) * 32 + lane;
       const int cols = BN / a.split;                                        // this CTA's columns of the tile
-      const uint32_t base = smem_u32(smem);
-      for (int c = (warp - 4) >> 2; c < cols; c += EPI / 4) {
+      const uint32_t base = smem_u32(smem) + row * 4;
+      constexpr int kAtOnce = BN / 4 < 8 ? BN / 4 : 8;                      // columns of a thread at a time (split <= 4)
+      for (int c = (warp - 4) / 4 * kAtOnce; c < cols; c += EPI / 4 * kAtOnce) {
         const int col = part * cols + c;
-        float v = 0.0f;
-        for (int s = 0; s < a.split; ++s) v += load_cluster(map_to_cta(base + (col * 128 + row) * 4, s));
-        if (t.p0 + row < a.p_rows && t.q0 + col < a.q_rows) store_one<SWAP>(a, t.p0 + row, t.q0 + col, v);
+        float v[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) v[j] = 0.0f;
+        for (int s = 0; s < a.split; ++s) {
+          float w[kAtOnce];
+          const uint32_t from = map_to_cta(base + col * 512, s);
+#pragma unroll
+          for (int j = 0; j < kAtOnce; ++j) w[j] = load_cluster(from + j * 512);
+#pragma unroll
+          for (int j = 0; j < kAtOnce; ++j) v[j] += w[j];
+        }
+        if (t.p0 + row < a.p_rows) {
+          if constexpr (SWAP) {
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+              if (t.q0 + col + j < a.q_rows) store_one<true>(a, t.p0 + row, t.q0 + col + j, v[j]);
+          } else {
+            store_row<kAtOnce>(a, t.p0 + row, t.q0 + col, v);
+          }
+        }
       }
     }
     __syncwarp();
@@ -748,11 +766,11 @@ int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMa
     set_error("wm_fp8_matmul: more than 2^30 tiles");
     return WM_ERR_INVALID;
   }
-  // Few tiles: 2, 4 or 8 CTAs take a share of the blocks each, while every SM still gets at most one CTA
-  // and every CTA two blocks.
+  // Few tiles: 2 or 4 CTAs take a share of the blocks each, while every SM still gets at most one CTA and every CTA
+  // two blocks.  (Clusters of 8 start 2 us later: 1 x 2048 x 4096 took 10.0 us with them, 7.4 us with 4.)
   a.split = 1;
   if (!PAIR)
-    while (a.split < 8 && tiles * a.split * 2 <= sms && a.kblocks / (a.split * 2) >= 2) a.split *= 2;
+    while (a.split < 4 && tiles * a.split * 2 <= sms && a.kblocks / (a.split * 2) >= 2) a.split *= 2;
   const int group = PAIR ? 2 : a.split;
   const long long groups = tiles * group <= sms ? tiles : sms / group;
   cudaLaunchConfig_t config{};
@@ -767,7 +785,7 @@ int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMa
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attributes;
-  config.numAttrs = PAIR && a.findings != nullptr ? 2 : 1;   // early only behind the packing kernel
+  config.numAttrs = 2;
   WM_CUDA(cudaLaunchKernelEx(&config, kernel, tp, tq, tout, tsp, tsq, a));
   count_launch();
   return WM_OK;
@@ -853,8 +871,8 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   }
   const bool by_column = a.q_shift == 0;
   if (bn == 16) return launch_matmul<16, 4, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
-  if (bn == 32) return launch_matmul<32, 4, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
-  if (bn == 64) return launch_matmul<64, 4, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
+  if (bn == 32) return launch_matmul<32, 8, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
+  if (bn == 64) return launch_matmul<64, 8, true, true, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
   if (pairs)
     return by_column ? launch_matmul<256, 8, false, true, true>(tp, tq, tout, tsp, tsq, a, sms, stream)
                      : launch_matmul<256, 8, false, false, true>(tp, tq, tout, tsp, tsq, a, sms, stream);
