@@ -219,7 +219,7 @@ WM_API int wm_route_plan(int32_t phase, int32_t world, int32_t rank, int32_t exp
  *   quantises x^T.  Output q is [batches][m][ceil128(k)] bytes (padding bytes written), scales
  *   [batches][ceil(m / block_rows)][ceil(k / 128)] with (m, k) = transpose ? (cols, rows) : (rows, cols).
  * wm_fp8_quantize_both: the 1 x 128 blocks of x (q, s) and of x^T (qt, st), bits as of two wm_fp8_quantize calls; one
- *   read of x where it is BF16 with cols % 8 == 0 and aligned (x and qt 16 bytes, q 8).
+ *   read of x where it is BF16 and the outputs are aligned (qt 16 bytes, q 8).
  * wm_fp8_quantize_weight: one read of each 128 x 128 block, emits W (q, s) and W^T (qt, st) with the
  *   same bytes and scales.  Operands must not alias; FP8 outputs must be 4-byte aligned.
  * wm_fp8_transpose_weight: byte transpose of a 128 x 128-quantised weight, bits preserved. */

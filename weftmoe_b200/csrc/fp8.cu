@@ -170,11 +170,12 @@ __global__ void quantize_rows_bf16_kernel(const uint4* __restrict__ x, long long
 }
 
 // 1 x 128 blocks of BF16 x along its columns (q, s) and along its rows (qt, st: the blocks of x^T), either of
-// them optional, from one read.  HBM-bound: 2 + 1 + 1 bytes an element.  One CTA per 128 x 128 tile; cols % 8 == 0 and
-// 16-byte aligned rows.  A row's block lies in 16 lanes and is quantised in registers; for the columns the tile passes
+// them optional, from one read.  HBM-bound: 2 + 1 + 1 bytes an element.  One CTA per 128 x 128 tile.  WIDE: cols % 8 == 0
+// and 16-byte aligned rows, read 16 bytes at a time; otherwise element by element.  A row's block lies in 16 lanes and is quantised in registers; for the columns the tile passes
 // through shared memory, and a thread takes two columns of 32 rows, so that it writes whole 32-byte sectors of qt.
 // Magnitudes are compared as their bit patterns, in which infinities and NaN come out on top.
-// 8192 x 2048, both: 15 us where two passes over x took 124 us.
+// 8192 x 2048, both: 19 us where two passes over x took 124 us.
+template <bool WIDE>
 __global__ void __launch_bounds__(256) quantize_both_bf16_kernel(const __nv_bfloat16* __restrict__ x, int rows, int cols,
                                                                  unsigned char* __restrict__ q, float* __restrict__ s,
                                                                  unsigned char* __restrict__ qt, float* __restrict__ st) {
@@ -188,9 +189,21 @@ __global__ void __launch_bounds__(256) quantize_both_bf16_kernel(const __nv_bflo
   const __nv_bfloat16* from = x + (batch * rows + r0 + line) * static_cast<size_t>(cols) + c0 + sub * 8;
   uint4 raw[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    raw[i] = in_cols && r0 + i * 16 + line < rows
-                 ? __ldg(reinterpret_cast<const uint4*>(from + static_cast<size_t>(i * 16) * cols)) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < 8; ++i) {
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (!in_cols || r0 + i * 16 + line >= rows) continue;
+    const __nv_bfloat16* piece = from + static_cast<size_t>(i * 16) * cols;
+    if constexpr (WIDE) {
+      raw[i] = __ldg(reinterpret_cast<const uint4*>(piece));
+    } else {
+      const unsigned short* each = reinterpret_cast<const unsigned short*>(piece);
+      const int left = cols - (c0 + sub * 8);
+      unsigned w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = j < left ? __ldg(each + j) : 0;
+      raw[i] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+  }
   if (qt != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) tile[(i * 16 + line) * 16 + sub] = raw[i];
@@ -302,13 +315,15 @@ int launch_tile(const void* x, int batches, int rows, int cols, int mode, void* 
 }
 
 // Whether quantize_both_bf16_kernel takes these operands.
-bool fits_both(const void* x, int dtype, int cols, const void* q, const void* qt) {
-  return dtype == 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(q) % 8 == 0 && reinterpret_cast<uintptr_t>(qt) % 16 == 0;
+bool fits_both(const void* x, int dtype, int rows, const void* q, const void* qt) {
+  return dtype == 0 && reinterpret_cast<uintptr_t>(x) % 2 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
+         reinterpret_cast<uintptr_t>(qt) % 16 == 0 && (rows + 127) / 128 <= 65535;
 }
 int launch_both(const void* x, int batches, int rows, int cols, void* q, float* s, void* qt, float* st,
                 cudaStream_t stream) {
-  quantize_both_bf16_kernel<<<dim3((cols + 127) / 128, (rows + 127) / 128, batches), 256, 0, stream>>>(
+  const bool wide = cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  auto kernel = wide ? quantize_both_bf16_kernel<true> : quantize_both_bf16_kernel<false>;
+  kernel<<<dim3((cols + 127) / 128, (rows + 127) / 128, batches), 256, 0, stream>>>(
       static_cast<const __nv_bfloat16*>(x), rows, cols, static_cast<unsigned char*>(q), s,
       static_cast<unsigned char*>(qt), st);
   WM_CUDA(cudaGetLastError());
@@ -381,8 +396,10 @@ extern "C" int wm_fp8_quantize(const void* x, int32_t dtype, int32_t batches, in
     count_launch();
     return WM_OK;
   }
-  if (block_rows == 1 && transpose && fits_both(x, dtype, cols, nullptr, q) && (rows + 127) / 128 <= 65535)
+  if (block_rows == 1 && transpose && fits_both(x, dtype, rows, nullptr, q))
     return launch_both(x, batches, rows, cols, nullptr, nullptr, q, scales, stream);
+  if (block_rows == 1 && !transpose && fits_both(x, dtype, rows, q, nullptr))
+    return launch_both(x, batches, rows, cols, q, scales, nullptr, nullptr, stream);
   // x^T with 128 x 128 blocks is the transposed output of the block mode.
   const int mode = block_rows == 128 ? kBlock : (transpose ? kRowsOfTranspose : kRows);
   void* qa = transpose ? nullptr : q;
@@ -401,7 +418,7 @@ extern "C" int wm_fp8_quantize_both(const void* x, int32_t dtype, int32_t batche
     set_error("wm_fp8_quantize_both: null output, or FP8 output data that is not 4-byte aligned");
     return WM_ERR_INVALID;
   }
-  if (fits_both(x, dtype, cols, q, qt) && (rows + 127) / 128 <= 65535)
+  if (fits_both(x, dtype, rows, q, qt))
     return launch_both(x, batches, rows, cols, q, s, qt, st, static_cast<cudaStream_t>(stream_));
   if (int rc = wm_fp8_quantize(x, dtype, batches, rows, cols, 1, 0, q, s, stream_)) return rc;
   return wm_fp8_quantize(x, dtype, batches, rows, cols, 1, 1, qt, st, stream_);

@@ -255,8 +255,9 @@ __device__ __forceinline__ void store_row(const MatmulArgs& a, int p, int q, con
   for (int j = 0; j < COLS; ++j)
     if (q + j < a.q_rows) store_one<false>(a, p, q + j, v[j]);
 }
-// A warp's 32 rows x 2 * PAIRS columns through shared memory and TMA: boxes of 32 rows x 128 bytes, 16-byte pieces
-// swizzled by the row as the map says.  The tensor map clips what lies outside the matrix.
+// A warp's 32 rows x 2 * PAIRS columns by way of shared memory: boxes of 32 rows x 128 bytes, 16-byte pieces swizzled by
+// the row.  From there TMA writes them (tma_store; the map clips what lies outside the matrix), or, where the rows of out are
+// not aligned or are added to, the warp does, row by row: 64 or 128 neighbouring bytes an instruction.
 template <int PAIRS>
 __device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorMap* tmap, uint8_t* staging, int p, int q,
                                             int lane, const uint64_t (&sum)[PAIRS]) {
@@ -265,7 +266,7 @@ __device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorM
 #pragma unroll
   for (int b = 0; b < PAIRS / 16; ++b) {
     if (b == boxes) break;
-    if (lane == 0) bulk_wait_group_read<0>();            // the box before this one has left the staging
+    if (a.tma_store && lane == 0) bulk_wait_group_read<0>();   // the box before this one has left the staging
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
@@ -282,12 +283,35 @@ __device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorM
       }
       *reinterpret_cast<uint4*>(line + ((c ^ (lane & 7)) << 4)) = w;
     }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      const int x = q + b * (a.out_is_f32 ? 32 : 64);
-      if (p < a.p_rows && x < a.q_rows) tma_store_2d(tmap, staging, x, p);
-      bulk_commit_group();
+    const int x = q + b * (a.out_is_f32 ? 32 : 64);
+    if (a.tma_store) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (p < a.p_rows && x < a.q_rows) tma_store_2d(tmap, staging, x, p);
+        bulk_commit_group();
+      }
+    } else {
+      __syncwarp();
+      const int rows = min(32, a.p_rows - p);
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) {
+        const long long at = static_cast<long long>(p + r) * a.ld + x + lane;
+        if (a.out_is_f32) {
+          const float w = *reinterpret_cast<const float*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          float* o = static_cast<float*>(a.out) + at;
+          if (x + lane < a.q_rows) *o = a.accumulate ? *o + w : w;
+        } else {
+          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = lane + 32 * h;
+            const uint8_t* from = staging + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2;
+            if (x + col < a.q_rows) o[32 * h] = *reinterpret_cast<const __nv_bfloat16*>(from);
+          }
+        }
+      }
+      __syncwarp();
     }
   }
 }
@@ -609,21 +633,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
           if (p0 + row < a.p_rows && t.q0 + col0 + 2 * j + 1 < a.q_rows)
             store_one<true>(a, p0 + row, t.q0 + col0 + 2 * j + 1, w.y);
         }
-      } else if (a.tma_store) {
+      } else {
         store_boxes<kCols / 2>(a, &tmap_out, smem + S::kStages * S::kStageBytes + (warp - 4) * S::kStoreBytes,
                                p0 + q * 32, t.q0 + col0, lane, sum);
-      } else if (p0 + row < a.p_rows) {
-#pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) {
-          float w[32];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 h = halves_of(sum[c * 16 + j]);
-            w[2 * j] = h.x;
-            w[2 * j + 1] = h.y;
-          }
-          store_row<32>(a, p0 + row, t.q0 + col0 + c * 32, w);
-        }
       }
     }
     if (!SWAP && lane == 0) bulk_wait_group_read<0>();   // the staging stays until it is read
