@@ -319,7 +319,7 @@ WM_API int wm_scatter_output(const void* output, int32_t tokens, int32_t start, 
  * Balance loss: mean over the sequences that have a live token of sum_e f_e P_e; f_e = experts * counts_e / sum of
  * counts, P_e = mean over live tokens of score_e / (sum of the token's scores).  Its gradient takes counts as given.
  * Results do not depend on the order in which blocks run.  No call synchronises or allocates; all may be captured.
- * experts <= 1024, top_k <= 32, num_sequences <= 65535. */
+ * tokens < 2^26, experts <= 1024, top_k <= 32, num_sequences <= 65535. */
 typedef struct wm_router {
   const void* logits;
   int64_t row_stride;       /* elements, >= experts                                                */

@@ -70,6 +70,43 @@ def test_shared_tiles_and_long_grids(m, n, k, b_rows):
     check(m, n, k, 1, b_rows, torch.bfloat16, seed=5)
 
 
+@pytest.mark.parametrize("b_rows", (1, 128))
+@pytest.mark.parametrize("blocks", (1, 7, 8, 9, 31, 32, 33, 65))
+def test_scales_on_the_tensor_cores(blocks, b_rows):
+    """Large tiles with power-of-two scales, up to and beyond one group of 32 blocks and one of the packing kernel;
+    a short last block; then the same with one scale that is no power of two, one zero and one NaN."""
+    m, n, k = 1500, 1700, blocks * 128 - 5
+    a, b = operand(m, k, 1, 50), operand(n, k, b_rows, 51)
+    want = wide(a) @ wide(b).t()
+    assert torch.equal(fp8_matmul(a, b, dtype=torch.float32), want.float())
+    for value in (1.5, 0.0):
+        b.scales[-1, -1] = value
+        assert torch.equal(fp8_matmul(a, b, dtype=torch.float32), (wide(a) @ wide(b).t()).float())
+    a.scales[77, 0] = float("nan")
+    got = fp8_matmul(a, b)
+    assert torch.isnan(got[77]).all() and not torch.isnan(got[:77]).any() and not torch.isnan(got[78:]).any()
+
+
+def test_far_powers_of_two_on_the_tensor_cores():
+    a, b = operand(1500, 1100, 1, 52), operand(1700, 1100, 128, 53)
+    a.scales[:, 0], b.scales[:, 0] = 2.0 ** 100, 2.0 ** -101
+    a.scales[:, 1], b.scales[:, 1] = 2.0 ** -60, 2.0 ** 62
+    assert torch.equal(fp8_matmul(a, b, dtype=torch.float32), (wide(a) @ wide(b).t()).float())
+
+
+@pytest.mark.parametrize("k", (4096, 16000))
+def test_random_products_on_the_tensor_cores(k):
+    """Quantised values: the accumulator cuts at most 2 U of what it holds at each of a group's 128 steps, so the bound of
+    the general form holds here too.  In the mean square: a cut is U of the accumulator on average, always towards zero, and
+    the accumulator of a group grows as the root of its steps (2/3 of its end on average): 128 * 2/3 * U = 2^-17.6."""
+    a = quantize_fp8(torch.randn(1500, k, device="cuda", generator=generator(54)).bfloat16())
+    b = quantize_fp8(torch.randn(1700, k, device="cuda", generator=generator(55)).bfloat16(), block_rows=128)
+    want, terms = wide(a) @ wide(b).t(), wide(a).abs() @ wide(b).abs().t()
+    got = fp8_matmul(a, b, dtype=torch.float32).double()
+    assert ((got - want).abs() <= (256 + -(-k // 128) + 2) * U * terms).all()
+    assert (got - want).norm() <= 2.0 ** -17.5 * want.norm()
+
+
 @pytest.mark.parametrize("m, n, k", [(1, 512, 2048), (33, 700, 1100), (200, 300, 4097), (700, 1300, 2000)])
 @pytest.mark.parametrize("a_rows, b_rows", [(1, 1), (1, 128), (128, 128)])
 def test_any_scales(m, n, k, a_rows, b_rows):
@@ -170,6 +207,44 @@ def test_captured_twice_and_on_another_stream():
     for small, large in outs:
         assert torch.equal(small, want) and torch.equal(large, want_big)
     poll_fp8_matmul()
+
+
+@pytest.mark.parametrize("m", (16, 1500))
+def test_captured_behind_copies_clears_and_joins(m):
+    """A product may start its prologue under the kernel before it: here what is before it is a memory copy, a clear,
+    another stream's work, or a kernel that writes its operands."""
+    host = torch.randn(m, 1024).bfloat16().pin_memory()
+    x = torch.empty(m, 1024, device="cuda", dtype=torch.bfloat16)
+    w = quantize_fp8(torch.randn(1700, 1024, device="cuda").bfloat16(), block_rows=128)
+    out = torch.empty(m, 1700, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step():
+        x.copy_(host, non_blocking=True)
+        a = quantize_fp8(x)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = fp8_matmul(a, w)
+        out.zero_()
+        fp8_matmul(a, w, dtype=torch.float32, out=out, accumulate=True)
+        torch.cuda.current_stream().wait_stream(side)
+        fp8_matmul(a, w, dtype=torch.float32, out=out, accumulate=True)
+        return other
+
+    side.wait_stream(torch.cuda.current_stream())
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other = step()
+    for seed in (1, 2):
+        host.copy_(torch.randn(m, 1024, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        a = quantize_fp8(host.cuda())
+        once = fp8_matmul(a, w, dtype=torch.float32)
+        assert torch.equal(out, 2 * once) and torch.equal(other, fp8_matmul(a, w))
+    del graph
 
 
 def test_offsets_beyond_32_bits():

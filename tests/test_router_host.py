@@ -19,6 +19,7 @@ LOGITS = torch.zeros(4, 8)
     (dict(logits=torch.zeros(2, 4, 8)), "BF16, FP32 or FP16"),
     (dict(logits=torch.zeros(4, 0)), "experts"),
     (dict(logits=torch.zeros(4, 1025)), "experts"),
+    (dict(logits=torch.zeros(1, 1).expand(2 ** 26, 1)), "tokens"),
     (dict(top_k=0), "top_k"),
     (dict(top_k=9), "top_k"),
     (dict(logits=torch.zeros(4, 64), top_k=33), "top_k"),
@@ -54,6 +55,8 @@ def test_counts_refusals():
     for bad in (routes.long(), routes[0], routes.t(), torch.zeros(4, 33, dtype=torch.int32)):
         with pytest.raises(ValueError, match="routes"):
             expert_counts(bad, 8)
+    with pytest.raises(ValueError, match="tokens"):
+        expert_counts(torch.empty((2 ** 26, 1), dtype=torch.int32, device="meta"), 8)
     for experts in (0, 1025, 8.0):
         with pytest.raises(ValueError, match="experts"):
             expert_counts(routes, experts)
@@ -85,7 +88,7 @@ def test_c_entries_refuse_before_any_device_work():
     lib = _lib.load()
     size = ctypes.c_int64()
     for change in (dict(experts=0), dict(experts=1025, row_stride=1025), dict(dtype=3), dict(row_stride=7),
-                   dict(score=2), dict(tokens=-1), dict(logits=None), dict(num_sequences=2),
+                   dict(score=2), dict(tokens=-1), dict(tokens=2 ** 26), dict(logits=None), dict(num_sequences=2),
                    dict(sequences=64, num_sequences=0), dict(sequences=64, num_sequences=65536)):
         r = _description(**change)
         assert lib.wm_router_workspace(ctypes.byref(r), ctypes.byref(size)) == _lib.WM_ERR_INVALID, change

@@ -26,6 +26,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kFinishWarps = 32;
 constexpr int kMaxExperts = 1024;
+constexpr int kMaxTokens = (1 << 26) - 1;   // x 32 routes: counts fit in 32 bits
 constexpr int kMaxBlocks = 1184;  // 148 SMs x 8
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -126,20 +127,27 @@ template <class T, int VEC>
 struct alignas(sizeof(T) * VEC) Piece {
   T v[VEC];
 };
+// A lane's part of a row as it is stored, so that the next row can be on its way while this one is worked on.
 template <class T, int V, int VEC>
-__device__ __forceinline__ void load_row(const Rows& a, long long row, int lane, float (&x)[V]) {
+struct RowPieces {
+  Piece<T, VEC> piece[V / VEC];
+};
+template <class T, int V, int VEC>
+__device__ __forceinline__ void fetch_row(const Rows& a, long long row, int lane, RowPieces<T, V, VEC>& r) {
   const T* p = static_cast<const T*>(a.logits) + row * a.stride;
 #pragma unroll
-  for (int j = 0; j < V; j += VEC) {
-    const int e = expert_of<VEC>(j, lane);
-    if (e < a.experts) {   // experts % VEC == 0: a piece is whole or absent
-      const Piece<T, VEC> w = *reinterpret_cast<const Piece<T, VEC>*>(p + e);
+  for (int j = 0; j < V / VEC; ++j) {
+    const int e = expert_of<VEC>(j * VEC, lane);   // experts % VEC == 0: a piece is whole or absent
+    if (e < a.experts) r.piece[j] = *reinterpret_cast<const Piece<T, VEC>*>(p + e);
+  }
+}
+template <class T, int V, int VEC>
+__device__ __forceinline__ void unpack_row(const Rows& a, int lane, const RowPieces<T, V, VEC>& r, float (&x)[V]) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[j + i] = as_float(w.v[i]);
-    } else {
+  for (int j = 0; j < V / VEC; ++j) {
+    const bool there = expert_of<VEC>(j * VEC, lane) < a.experts;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[j + i] = -INFINITY;
-    }
+    for (int i = 0; i < VEC; ++i) x[j * VEC + i] = there ? as_float(r.piece[j].v[i]) : -INFINITY;
   }
 }
 template <class T, int V, int VEC>
@@ -173,7 +181,7 @@ constexpr float kFar = -60.0f;   // sigmoids of a row with a logit above this ar
 // Of a row: its largest logit, whether an expert is available, and whether it has no distribution (NaN, or for
 // softmax +inf, among its logits).
 struct RowTop {
-  float top;
+  float top, lane_top;   // of the row, of this lane's part of it
   bool bad, any;
 };
 template <int V>
@@ -182,6 +190,7 @@ __device__ __forceinline__ RowTop row_top(const float (&x)[V], bool sigmoid) {
   float top = x[0];
 #pragma unroll
   for (int j = 1; j < V; ++j) top = max_or_nan(top, x[j]);
+  r.lane_top = top;
   r.bad = __any_sync(kAll, top != top);
   r.top = r.bad ? 0.0f : warp_max(top);
   r.bad |= !sigmoid && r.top == INFINITY;
@@ -281,18 +290,15 @@ __device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, 
   return expert;
 }
 
-// The K largest (value, lowest expert first) of the warp's V x 32 values; -inf is no candidate.  The (K+1)th largest
-// of the lanes' maxima is at most the (K+1)th largest value, so the values from it up hold the choice and the one
+// The K largest (value, lowest expert first) of the warp's V x 32 values, `most` the lane's largest; -inf is no
+// candidate.  The (K+1)th largest of the lanes' maxima is at most the (K+1)th largest value, so the values from it up hold the choice and the one
 // behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They, and with a margin what is at
 // most so much smaller, are gathered in `held` (32 of this warp), and each counts the ones before it.  Lane k gets choice
 // k and its value; `behind` the next value (-inf: none).  Returns the number of candidates, which stay in `held` in
 // their order; above 32 (many equal values) nothing is chosen.
 template <int V, int VEC>
-__device__ __forceinline__ int choose(const float (&x)[V], float margin, int top_k, int lane, float2* held, int& expert,
+__device__ __forceinline__ int choose(const float (&x)[V], float most, float margin, int top_k, int lane, float2* held, int& expert,
                                       float& its, float& behind) {
-  float most = x[0];
-#pragma unroll
-  for (int j = 1; j < V; ++j) most = fmaxf(most, x[j]);
   unsigned key = most > -INFINITY ? ordered(most) : 0u, border = 0;
   for (int k = 0; k <= top_k; ++k) {   // equal maxima go at once: the border is then lower, which is as good
     border = __reduce_max_sync(kAll, key);
@@ -318,12 +324,16 @@ __device__ __forceinline__ int choose(const float (&x)[V], float margin, int top
   for (int j = 0; j < V; ++j)
     if (x[j] >= from) held[at++] = make_float2(x[j], __int_as_float(expert_of<VEC>(j, lane)));
   __syncwarp();
-  float2 me = make_float2(-INFINITY, __int_as_float(0x7fffffff));
-  if (lane < n) me = held[lane];
+  if (lane >= n) held[lane] = make_float2(-INFINITY, __int_as_float(0x7fffffff));   // ranks behind all candidates
+  __syncwarp();
+  const float2 me = held[lane];
   int before = 0;
-  for (int i = 0; i < n; ++i) {
-    const float2 other = held[i];
-    before += other.x > me.x || (other.x == me.x && __float_as_int(other.y) < __float_as_int(me.y));
+  for (int i = 0; i < n; i += 4) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 other = held[i + w];
+      before += other.x > me.x || (other.x == me.x && __float_as_int(other.y) < __float_as_int(me.y));
+    }
   }
   __syncwarp();
   if (lane < n) held[before] = me;
@@ -372,7 +382,10 @@ __device__ __forceinline__ bool choose_by_score(const float (&x)[V], const float
     }
   }
   float mine, behind;
-  const int n = choose<V, VEC>(v, 2.0f * doubt, a.top_k, lane, held, expert, mine, behind);
+  float most = v[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) most = fmaxf(most, v[j]);
+  const int n = choose<V, VEC>(v, most, 2.0f * doubt, a.top_k, lane, held, expert, mine, behind);
   if (n > 32) return false;
   float next = __shfl_down_sync(kAll, mine, 1);
   int next_expert = __shfl_down_sync(kAll, expert, 1);
@@ -416,14 +429,15 @@ struct Records {
 
 // Blocks of an SM that the registers are shared out for.
 template <int V>
-constexpr int kResident = V <= 8 ? 4 : V <= 16 ? 2 : 1;
+constexpr int kResident = V <= 8 ? 4 : V <= 16 ? 3 : 1;
 
 template <class T, int V, int VEC>
 __global__ void __launch_bounds__(kWarps * 32, kResident<V>)
 router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict__ gates, const Records rec) {
-  extern __shared__ float smem[];
-  float* part = smem;                                              // [kWarps][experts]
-  int* seen = reinterpret_cast<int*>(smem + kWarps * a.experts);   // [experts]
+  extern __shared__ float4 smem_sums[];                            // (16-byte aligned)
+  float* part = reinterpret_cast<float*>(smem_sums);                                            // [kWarps][experts], each warp's sums of p
+  float* mine = part + (threadIdx.x >> 5) * a.experts;
+  int* seen = reinterpret_cast<int*>(part + kWarps * a.experts);   // [experts]
   __shared__ int live_rows[kWarps], live_routes[kWarps];
   __shared__ float2 held[kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -443,28 +457,40 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
   while (row0 < last) {
     const int b = sequence_of(a, row0);
     const int row1 = balance ? max(row0 + 1, min(last, sequence_end(a, b))) : last;
-    float acc[V];
+    if (balance) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < V; j += VEC) {
+        const int e = expert_of<VEC>(j, lane);
+        if (e < a.experts) *reinterpret_cast<Piece<float, VEC>*>(mine + e) = Piece<float, VEC>{};
+      }
+    }
     int rows = 0, taken = 0;
+    RowPieces<T, V, VEC> next;
+    if (row0 + warp < row1) fetch_row<T, V, VEC>(a, row0 + warp, lane, next);
     for (int row = row0 + warp; row < row1; row += kWarps) {
+      const RowPieces<T, V, VEC> here = next;
+      if (row + kWarps < row1) fetch_row<T, V, VEC>(a, row + kWarps, lane, next);
       int expert = -1;
       float weight = 0.0f;
       if (row_live(a, row, balance ? b : sequence_of(a, row))) {
         float x[V], h[V], rest[V];
-        load_row<T, V, VEC>(a, row, lane, x);
+        unpack_row<T, V, VEC>(a, lane, here, x);
         const RowTop r = row_top<V>(x, a.sigmoid);
         float sum = 1.0f;
         if (whole && r.any && !r.bad) sum = row_shares<V>(x, a.sigmoid, r.top, h, rest);
         if (balance && (r.any || r.bad)) {
           ++rows;
-          if (r.bad) {
+          const float inv = 1.0f / sum;
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] = NAN;
-          } else {
-            const float inv = 1.0f / sum;
+          for (int j = 0; j < V; j += VEC) {
+            const int e = expert_of<VEC>(j, lane);
+            if (e < a.experts) {
+              Piece<float, VEC>& w = *reinterpret_cast<Piece<float, VEC>*>(mine + e);
+              Piece<float, VEC> acc = w;
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] = fmaf(h[j], inv, acc[j]);
+              for (int i = 0; i < VEC; ++i) acc.v[i] = r.bad ? NAN : fmaf(h[j + i], inv, acc.v[i]);
+              w = acc;
+            }
           }
         }
         if (pick && r.bad) {   // no distribution: valid routes and NaN gates, so that it shows in the output
@@ -478,7 +504,7 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
             settled = choose_by_score<T, V, VEC>(x, h, sum, a, logits, r.top, lane, held[warp], expert);
             if (settled && expert >= 0) logit = as_float(logits[expert]);
           } else {
-            settled = choose<V, VEC>(x, 0.0f, a.top_k, lane, held[warp], expert, logit, behind) <= 32;
+            settled = choose<V, VEC>(x, r.lane_top, 0.0f, a.top_k, lane, held[warp], expert, logit, behind) <= 32;
           }
           if (!settled) {
             expert = choose_slowly<T>(logits, a.experts, a.top_k, a.bias, a.sigmoid != 0, r.top, lane);
@@ -494,11 +520,6 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
       }
     }
     if (balance) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = expert_of<VEC>(j, lane);
-        if (e < a.experts) part[warp * a.experts + e] = acc[j];
-      }
       taken = __reduce_add_sync(kAll, taken);
       if (lane == 0) { live_rows[warp] = rows; live_routes[warp] = taken; }
       __syncthreads();
@@ -639,11 +660,15 @@ router_backward_kernel(const Rows a, const int* __restrict__ routes, const float
   const long long from = (static_cast<long long>(blockIdx.x) * kWarps + warp) * a.chunk;
   const int end = static_cast<int>(min(from + a.chunk, static_cast<long long>(a.tokens)));
   int b = 0, b_end = -1;
+  RowPieces<T, V, VEC> next;
+  if (from < end) fetch_row<T, V, VEC>(a, from, lane, next);
   for (int row = static_cast<int>(min(from, static_cast<long long>(a.tokens))); row < end; ++row) {
     if (row >= b_end) {
       b = sequence_of(a, row);
       b_end = max(row + 1, sequence_end(a, b));
     }
+    const RowPieces<T, V, VEC> here = next;
+    if (row + 1 < end) fetch_row<T, V, VEC>(a, row + 1, lane, next);
     float d[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.0f;
@@ -658,7 +683,7 @@ router_backward_kernel(const Rows a, const int* __restrict__ routes, const float
         if (expert >= 0) logit = as_float((static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.stride)[expert]);
       }
       float x[V], h[V], rest[V];
-      load_row<T, V, VEC>(a, row, lane, x);
+      unpack_row<T, V, VEC>(a, lane, here, x);
       const RowTop r = row_top<V>(x, a.sigmoid);
       if (r.bad) {
 #pragma unroll
@@ -813,11 +838,11 @@ Plan plan_of(const wm_router& r) {
 
 int check_rows(const char* what, const wm_router* r) {
   if (!r) { set_error("%s: null arguments", what); return WM_ERR_INVALID; }
-  if (r->tokens < 0 || r->experts < 1 || r->experts > kMaxExperts || r->dtype < 0 || r->dtype > 2 ||
+  if (r->tokens < 0 || r->tokens > kMaxTokens || r->experts < 1 || r->experts > kMaxExperts || r->dtype < 0 || r->dtype > 2 ||
       r->row_stride < r->experts || (r->score != 0 && r->score != 1) || (r->tokens > 0 && !r->logits) ||
       (r->sequences ? r->num_sequences < 1 : r->num_sequences != 0) || r->num_sequences > 65535) {
-    set_error("%s: logits must be [tokens][experts] BF16 / FP32 / FP16 rows of 1..%d experts, score 0 (softmax) or 1 "
-              "(sigmoid), 1..65535 sequences with their offsets", what, kMaxExperts);
+    set_error("%s: logits must be [fewer than 2^26 tokens][experts] BF16 / FP32 / FP16 rows of 1..%d experts, score 0 (softmax) "
+              "or 1 (sigmoid), 1..65535 sequences with their offsets", what, kMaxExperts);
     return WM_ERR_INVALID;
   }
   return WM_OK;
@@ -976,9 +1001,9 @@ extern "C" int wm_router_backward(const wm_router* r, const int32_t* routes, con
 
 extern "C" int wm_expert_counts(const int32_t* routes, int32_t tokens, int32_t top_k, int32_t experts,
                                 const int32_t* sequences, int32_t num_sequences, int32_t* counts, void* stream_) {
-  if (tokens < 0 || top_k < 1 || top_k > 32 || experts < 1 || experts > kMaxExperts || !counts ||
+  if (tokens < 0 || tokens > kMaxTokens || top_k < 1 || top_k > 32 || experts < 1 || experts > kMaxExperts || !counts ||
       (tokens > 0 && !routes) || (sequences ? num_sequences < 1 : num_sequences != 0) || num_sequences > 65535) {
-    set_error("wm_expert_counts: routes [tokens][1..32], 1..%d experts, 1..65535 sequences with their offsets",
+    set_error("wm_expert_counts: routes [fewer than 2^26 tokens][1..32], 1..%d experts, 1..65535 sequences with their offsets",
               kMaxExperts);
     return WM_ERR_INVALID;
   }

@@ -26,6 +26,7 @@ _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 _SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
+MAX_TOKENS = 2 ** 26 - 1
 MAX_SEQUENCES = 65535
 
 
@@ -34,6 +35,8 @@ def _check_logits(logits):
         raise ValueError("logits must be a BF16, FP32 or FP16 tensor [tokens, experts]")
     if not 1 <= logits.shape[1] <= MAX_EXPERTS:
         raise ValueError(f"logits must have 1 to {MAX_EXPERTS} experts")
+    if logits.shape[0] > MAX_TOKENS:
+        raise ValueError(f"logits must have at most {MAX_TOKENS} tokens")
 
 
 def _check_vector(tensor, what, dtypes, length, like):
@@ -253,6 +256,8 @@ def expert_counts(routes, experts, *, sequences=None):
         raise ValueError("routes must be an int32 tensor [tokens, top_k]")
     if not 1 <= routes.shape[1] <= MAX_TOP_K or not routes.is_contiguous():
         raise ValueError(f"routes must be contiguous, with 1 to {MAX_TOP_K} columns")
+    if routes.shape[0] > MAX_TOKENS:
+        raise ValueError(f"routes must have at most {MAX_TOKENS} tokens")
     if not isinstance(experts, int) or not 1 <= experts <= MAX_EXPERTS:
         raise ValueError(f"experts must be in [1, {MAX_EXPERTS}]")
     _check_sequences(sequences, routes)
