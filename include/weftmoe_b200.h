@@ -256,6 +256,11 @@ WM_API int wm_fp8_matmul(const void* aq, const float* as, const void* bq, const 
                          void* stream);
 /* Bytes of the workspace a product of these sizes can use on the current device; 0 where it uses none. */
 WM_API int wm_fp8_matmul_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes);
+/* out[rows][n] = x W^T in one call: wm_fp8_quantize of x [rows][k] (1 x 128 blocks; BF16, or FP32 with x_is_f32, and out
+ * of x's type) into the workspace, then wm_fp8_matmul with the weight [n][k] in 128 x 128 blocks. */
+WM_API int wm_fp8_linear(const void* x, int32_t x_is_f32, int32_t rows, int32_t k, const void* wq, const float* ws,
+                         int32_t n, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+WM_API int wm_fp8_linear_workspace(int32_t rows, int32_t n, int32_t k, int64_t* bytes);
 WM_API int wm_fp8_matmul_status(int32_t* code, void* stream);
 
 /* ------------------------------------------------------------------------------------------

@@ -27,6 +27,16 @@ def test_nothing_to_do_touches_nothing(change):
     assert _lib.load().wm_fp8_matmul(*{**GOOD, **change}.values(), None) == _lib.WM_OK
 
 
+def test_linear_entry_refuses():
+    lib = _lib.load()
+    for rows, k, n in ((-1, 128, 8), (4, -1, 8), (4, 128, -1)):
+        assert lib.wm_fp8_linear(256, 0, rows, k, 256, 64, n, 64, 256, 1 << 20, None) == _lib.WM_ERR_INVALID
+    assert lib.wm_fp8_linear(None, 0, 0, 128, None, None, 8, None, None, 0, None) == _lib.WM_OK
+    size = ctypes.c_int64()
+    assert lib.wm_fp8_matmul_workspace(-1, 1, 1, ctypes.byref(size)) == _lib.WM_ERR_INVALID
+    assert lib.wm_fp8_linear_workspace(1, 1, -1, ctypes.byref(size)) == _lib.WM_ERR_INVALID
+
+
 def test_status_entry_refuses_a_null_result():
     assert _lib.load().wm_fp8_matmul_status(ctypes.POINTER(ctypes.c_int32)(), None) == _lib.WM_ERR_INVALID
 

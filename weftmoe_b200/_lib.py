@@ -80,6 +80,9 @@ SIGNATURES = {
     "wm_fp8_gemm": (c_int, [c_void_p] * 5 + [c_int32] * 7 + [c_void_p]),
     "wm_fp8_matmul": (c_int, [c_void_p] * 5 + [c_int64] + [c_int32] * 7 + [c_void_p, c_int64, c_void_p]),
     "wm_fp8_matmul_workspace": (c_int, [c_int32] * 3 + [POINTER(c_int64)]),
+    "wm_fp8_linear": (c_int, [c_void_p] + [c_int32] * 3 + [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64,
+                                                           c_void_p]),
+    "wm_fp8_linear_workspace": (c_int, [c_int32] * 3 + [POINTER(c_int64)]),
     "wm_fp8_matmul_status": (c_int, [POINTER(c_int32), c_void_p]),
     "wm_nvfp4_quantize": (c_int, [c_void_p, c_int32, c_int32, c_float, c_void_p, c_void_p, c_int32, c_void_p]),
     "wm_nvfp4_gemm": (c_int, [c_void_p] * 5 + [c_int32] * 3 + [c_float, c_int32, c_void_p]),

@@ -892,6 +892,37 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
                    : launch_matmul<128, 8, false, false, false>(tp, tq, tout, tsp, tsq, a, sms, stream);
 }
 
+extern "C" int wm_fp8_linear(const void* x, int32_t x_is_f32, int32_t rows, int32_t k, const void* wq, const float* ws,
+                             int32_t n, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (rows < 0 || k < 0 || n < 0) {
+    set_error("wm_fp8_linear: negative size");
+    return WM_ERR_INVALID;
+  }
+  if (rows == 0 || n == 0) return WM_OK;
+  const long long kblocks = (static_cast<long long>(k) + 127) / 128;
+  // the quantised x, its scales, the product's own workspace
+  const long long scales_at = static_cast<long long>(rows) * kblocks * 128;
+  const long long rest_at = (scales_at + static_cast<long long>(rows) * kblocks * 4 + 127) / 128 * 128;
+  int64_t rest = 0;
+  if (int rc = wm_fp8_matmul_workspace(rows, n, k, &rest)) return rc;
+  if (!workspace || workspace_bytes < rest_at + rest || reinterpret_cast<uintptr_t>(workspace) % 128) {
+    set_error("wm_fp8_linear: missing, small or misaligned workspace (wm_fp8_linear_workspace, 128-byte aligned)");
+    return WM_ERR_INVALID;
+  }
+  char* room = static_cast<char*>(workspace);
+  float* xs = reinterpret_cast<float*>(room + scales_at);
+  if (int rc = wm_fp8_quantize(x, x_is_f32, 1, rows, k, 1, 0, room, xs, stream)) return rc;
+  return wm_fp8_matmul(room, xs, wq, ws, out, n, rows, n, k, 1, 128, x_is_f32, 0, rest ? room + rest_at : nullptr, rest,
+                       stream);
+}
+
+extern "C" int wm_fp8_linear_workspace(int32_t rows, int32_t n, int32_t k, int64_t* bytes) {
+  if (int rc = wm_fp8_matmul_workspace(rows, n, k, bytes)) return rc;
+  const long long kblocks = (static_cast<long long>(k) + 127) / 128;
+  *bytes += (static_cast<long long>(rows) * kblocks * 132 + 127) / 128 * 128;
+  return WM_OK;
+}
+
 extern "C" int wm_fp8_matmul_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes) {
   if (m < 0 || n < 0 || k < 0 || !bytes) {
     set_error("wm_fp8_matmul_workspace: negative size or null result");

@@ -437,18 +437,38 @@ def prepare_fp8_linear(weight, *, training: bool = True) -> PreparedFP8Linear:
     return PreparedFP8Linear(straight, flipped, _ParameterStamp(weight))
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace_bytes(rows, n, k, device):
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().wm_fp8_linear_workspace(rows, n, k, ctypes.byref(size)))
+    return size.value
+
+
+def _linear_forward(x, weight):
+    """x W^T of a matrix x and a weight in 128 x 128 blocks: quantising and product in one call."""
+    device = x.device
+    rows, k = x.shape
+    n = weight.shape[0]
+    y = x.new_empty((rows, n))
+    size = _linear_workspace_bytes(rows, n, k, device.index)
+    workspace = x.new_empty(size, dtype=torch.uint8)
+    _lib.check(_lib.load().wm_fp8_linear(
+        x.data_ptr(), x.dtype == torch.float32, rows, k, weight.data.data_ptr(), weight.scales.data_ptr(), n, y.data_ptr(),
+        workspace.data_ptr(), size, stream_of(device, x, weight.data, weight.scales)))
+    return y
+
+
 class _FP8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, prepared):
         ctx.prepared, ctx.x_type = prepared, x.dtype
-        held = ()
-        if ctx.needs_input_grad[1]:             # kept for dW instead of x: the blocks along the tokens, a byte each
-            rows, columns = _quantize_fp8_both(x)
-            held = (columns.data, columns.scales)
-            ctx.columns_shape = columns.shape
-        else:
-            rows = quantize_fp8(x)
-        ctx.save_for_backward(weight, *held)    # the weight: detects optimizer updates before backward
+        # the weight is saved to detect optimizer updates before backward
+        if not ctx.needs_input_grad[1]:
+            ctx.save_for_backward(weight)
+            return _linear_forward(x, prepared.weight)
+        rows, columns = _quantize_fp8_both(x)   # kept for dW instead of x: the blocks along the tokens, a byte each
+        ctx.columns_shape = columns.shape
+        ctx.save_for_backward(weight, columns.data, columns.scales)
         return fp8_matmul(rows, prepared.weight, dtype=x.dtype)
 
     @staticmethod
@@ -496,5 +516,5 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, prepared: PreparedFP8Linea
         if training:
             y = _FP8Linear.apply(rows, weight, prepared)
         else:
-            y = fp8_matmul(quantize_fp8(rows), prepared.weight, dtype=x.dtype)
+            y = _linear_forward(rows, prepared.weight)
     return y if x.ndim == 2 else y.view(*x.shape[:-1], weight.shape[0])
