@@ -99,6 +99,8 @@ __device__ __forceinline__ float load_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Two FP32 multiply-adds in one instruction, on register pairs.
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
   uint64_t r;
@@ -651,16 +653,18 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
       constexpr int kAtOnce = BN / 4 < 8 ? BN / 4 : 8;                      // columns of a thread at a time (split <= 4)
       for (int c = (warp - 4) / 4 * kAtOnce; c < cols; c += EPI / 4 * kAtOnce) {
         const int col = part * cols + c;
-        float v[kAtOnce];
+        float v[kAtOnce], w[4][kAtOnce];                                      // all loads before the first addition
 #pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) v[j] = 0.0f;
-        for (int s = 0; s < a.split; ++s) {
-          float w[kAtOnce];
+        for (int s = 0; s < 4; ++s) {
+          if (s >= a.split) break;
           const uint32_t from = map_to_cta(base + col * 512, s);
 #pragma unroll
-          for (int j = 0; j < kAtOnce; ++j) w[j] = load_cluster(from + j * 512);
+          for (int j = 0; j < kAtOnce; ++j) w[s][j] = load_cluster(from + j * 512);
+        }
 #pragma unroll
-          for (int j = 0; j < kAtOnce; ++j) v[j] += w[j];
+        for (int j = 0; j < kAtOnce; ++j) {
+          v[j] = w[0][j] + w[1][j];                                           // split is 2 or 4
+          if (a.split == 4) v[j] = (v[j] + w[2][j]) + w[3][j];
         }
         if (t.p0 + row < a.p_rows) {
           if constexpr (SWAP) {
@@ -674,7 +678,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
       }
     }
     __syncwarp();
-    cluster_sync_all();   // the others' shared memory stays until it is read
+    cluster_arrive();
   }
   tc_fence_before();
   __syncthreads();
@@ -683,6 +687,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
     tc_fence_after();
     tmem_dealloc(tmem_base, S::kColumns);
   }
+  if (!PAIR && a.split > 1) cluster_wait();   // this CTA's sums stay until the others have read them
 }
 
 // FP32 scales -> UE8M0 chunks [ceil(rows / 128)][ceil(kblocks / 4)][512 bytes] in the 4 x 32 order of tcgen05.cp (word
