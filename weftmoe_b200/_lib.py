@@ -123,6 +123,17 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+def binding():
+    """The autograd edges in C++ (binding/torch_binding.cpp), on the same library; raise if they are not built."""
+    load()
+    try:
+        from . import _torch_binding
+    except ImportError as error:
+        raise RuntimeError(f"the autograd binding cannot be loaded ({error}): build it with "
+                           "`python -m weftmoe_b200.build`") from error
+    return _torch_binding
+
+
 def last_error() -> str:
     message = load().wm_last_error()
     return message.decode() if message else ""

@@ -10,6 +10,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -17,6 +18,9 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libweftmoe_b200.so"
 OBJECTS = PACKAGE / "build"
+
+BINDING_SOURCE = PACKAGE / "binding" / "torch_binding.cpp"
+BINDING = PACKAGE / ("_torch_binding" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -43,12 +47,42 @@ def _stale(target: Path, inputs: list[Path]) -> bool:
     return any(p.stat().st_mtime_ns > stamp for p in inputs)
 
 
+def _run(cmd, verbose=False):
+    if verbose:
+        print(" ".join(map(str, cmd)), flush=True)
+    done = subprocess.run(cmd, capture_output=True, text=True)
+    if done.returncode:
+        raise RuntimeError(f"build failed:\n{' '.join(map(str, cmd))}\n{done.stdout}\n{done.stderr}")
+    return done.stderr
+
+
+def _binding_command(obj):
+    """Host compilation of the autograd binding against the installed torch."""
+    import torch
+    root = Path(torch.__file__).resolve().parent / "include"
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda")) / "include"
+    includes = [root, root / "torch/csrc/api/include", sysconfig.get_paths()["include"], cuda]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_torch_binding",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *(f"-isystem{path}" for path in includes), "-c", str(BINDING_SOURCE), "-o", str(obj)]
+
+
+def _binding_link(obj):
+    import torch
+    libraries = Path(torch.__file__).resolve().parent / "lib"
+    return ["g++", "-shared", str(obj), "-o", str(BINDING), f"-L{libraries}", "-lc10", "-lc10_cuda", "-ltorch",
+            "-ltorch_cpu", "-ltorch_python", f"-L{PACKAGE}", f"-l:{LIBRARY.name}", "-Wl,-rpath,$ORIGIN"]
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile every .cu under csrc/ for sm_100a and link the shared library."""
+    """Compile every .cu under csrc/ for sm_100a, link the shared library, and build the autograd binding on it."""
     nvcc = _nvcc()
     headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + \
         sorted((PACKAGE.parent / "include").glob("*.h"))
     OBJECTS.mkdir(exist_ok=True)
+    binding = None
+    if force or _stale(BINDING, [BINDING_SOURCE, *headers]):   # host compiler, beside the kernels
+        binding = ThreadPoolExecutor(max_workers=1).submit(_run, _binding_command(OBJECTS / "torch_binding.o"), verbose)
     jobs = []
     for src in sources():
         obj = OBJECTS / (src.stem + ".o")
@@ -59,12 +93,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             jobs.append(cmd)
 
     def run(cmd):
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        done = subprocess.run(cmd, capture_output=True, text=True)
-        if done.returncode:
-            raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{done.stdout}\n{done.stderr}")
-        return done.stderr
+        return _run(cmd, verbose)
 
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as pool:
         logs = list(pool.map(run, jobs))
@@ -74,6 +103,9 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if force or jobs or _stale(LIBRARY, objects):
         run([nvcc, *ARCH_FLAGS, "-shared", "-o", str(LIBRARY), *map(str, objects),
              "-cudart", "static", "-Xcompiler", "-fPIC"])
+    if binding is not None:
+        binding.result()
+        run(_binding_link(OBJECTS / "torch_binding.o"))
     return LIBRARY
 
 

@@ -16,7 +16,6 @@ Storage rules:
 from __future__ import annotations
 
 import ctypes
-import functools
 import weakref
 from dataclasses import dataclass
 
@@ -191,14 +190,6 @@ def fp8_gemm(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Ten
     return out
 
 
-@functools.lru_cache(maxsize=1024)
-def _matmul_workspace_bytes(m, n, k, device):
-    """Room that a product of these sizes uses (0: none); `device` is the current one, whose SMs it depends on."""
-    size = ctypes.c_int64()
-    _lib.check(_lib.load().wm_fp8_matmul_workspace(m, n, k, ctypes.byref(size)))
-    return size.value
-
-
 def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.Tensor | None = None,
                accumulate: bool = False) -> torch.Tensor:
     """A @ B^T of A [M, K] and B [N, K], blocks of 1 or 128 rows on either side, any scales.
@@ -214,22 +205,14 @@ def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.T
     if accumulate and (out is None or dtype != torch.float32):
         raise ValueError("FP8 accumulation requires an existing FP32 output")
     (m, k), n = a.shape, b.shape[0]
-    device = a.data.device
-    with on_device(device):
-        if out is None:
-            out = a.scales.new_empty((m, n), dtype=dtype)
-        else:
-            fits = (isinstance(out, torch.Tensor) and tuple(out.shape) == (m, n) and out.dtype == dtype
-                    and out.device == device and (n <= 1 or out.stride(1) == 1) and (m <= 1 or out.stride(0) >= n))
-            if not fits:
-                raise ValueError("FP8 output shape, dtype, device or layout mismatch")
-        size = _matmul_workspace_bytes(m, n, k, device.index)
-        workspace = a.scales.new_empty(size, dtype=torch.uint8) if size else None
-        _lib.check(_lib.load().wm_fp8_matmul(
-            a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(), out.data_ptr(),
-            out.stride(0) if m > 1 else max(n, 1), m, n, k, a.block_rows, b.block_rows, int(dtype == torch.float32),
-            int(accumulate), None if workspace is None else workspace.data_ptr(), size, stream_of(device, a.data, a.scales, b.data, b.scales)))
-    return out
+    if out is not None:
+        fits = (isinstance(out, torch.Tensor) and tuple(out.shape) == (m, n) and out.dtype == dtype
+                and out.device == a.data.device and (n <= 1 or out.stride(1) == 1) and (m <= 1 or out.stride(0) >= n))
+        if not fits:
+            raise ValueError("FP8 output shape, dtype, device or layout mismatch")
+    product = _lib.binding().fp8_matmul(a.data, a.scales, a.block_rows, b.data, b.scales, b.block_rows, m, n, k,
+                                        dtype == torch.float32, out, accumulate)
+    return product if out is None else out
 
 
 def poll_fp8_matmul() -> None:
@@ -413,7 +396,7 @@ class PreparedFP8Linear:
             if self._ready.query():
                 self._ready = None
             else:
-                torch.cuda.current_stream().wait_event(self._ready)
+                torch.cuda.current_stream(self.weight.data.device).wait_event(self._ready)
 
 
 @torch.inference_mode(False)
@@ -437,61 +420,6 @@ def prepare_fp8_linear(weight, *, training: bool = True) -> PreparedFP8Linear:
     return PreparedFP8Linear(straight, flipped, _ParameterStamp(weight))
 
 
-@functools.lru_cache(maxsize=1024)
-def _linear_workspace_bytes(rows, n, k, device):
-    size = ctypes.c_int64()
-    _lib.check(_lib.load().wm_fp8_linear_workspace(rows, n, k, ctypes.byref(size)))
-    return size.value
-
-
-def _linear_forward(x, weight):
-    """x W^T of a matrix x and a weight in 128 x 128 blocks: quantising and product in one call."""
-    device = x.device
-    rows, k = x.shape
-    n = weight.shape[0]
-    y = x.new_empty((rows, n))
-    size = _linear_workspace_bytes(rows, n, k, device.index)
-    workspace = x.new_empty(size, dtype=torch.uint8)
-    _lib.check(_lib.load().wm_fp8_linear(
-        x.data_ptr(), x.dtype == torch.float32, rows, k, weight.data.data_ptr(), weight.scales.data_ptr(), n, y.data_ptr(),
-        workspace.data_ptr(), size, stream_of(device, x, weight.data, weight.scales)))
-    return y
-
-
-class _FP8Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, prepared):
-        ctx.prepared, ctx.x_type = prepared, x.dtype
-        # the weight is saved to detect optimizer updates before backward
-        if not ctx.needs_input_grad[1]:
-            ctx.save_for_backward(weight)
-            return _linear_forward(x, prepared.weight)
-        rows, columns = _quantize_fp8_both(x)   # kept for dW instead of x: the blocks along the tokens, a byte each
-        ctx.columns_shape = columns.shape
-        ctx.save_for_backward(weight, columns.data, columns.scales)
-        return fp8_matmul(rows, prepared.weight, dtype=x.dtype)
-
-    @staticmethod
-    def backward(ctx, dy):
-        if torch.is_grad_enabled():
-            raise RuntimeError("The gradients of fp8_linear cannot be differentiated again")
-        weight, *held = ctx.saved_tensors
-        to_x, to_weight, _ = ctx.needs_input_grad
-        dy = dy.contiguous()
-        dx = dweight = rows = columns = None
-        if to_x and to_weight:
-            rows, columns = _quantize_fp8_both(dy)
-        elif to_x:
-            rows = quantize_fp8(dy)
-        else:
-            columns = quantize_fp8(dy, transpose=True)
-        if to_x:
-            dx = fp8_matmul(rows, ctx.prepared.weight_t, dtype=ctx.x_type)
-        if to_weight:
-            dweight = fp8_matmul(columns, FP8Tensor(*held, ctx.columns_shape), dtype=weight.dtype)
-        return dx, dweight, None
-
-
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, prepared: PreparedFP8Linear) -> torch.Tensor:
     """y = x W^T for x [..., in] and W [out, in] on the FP8 tensor cores, the projection beside the FP8 experts.
 
@@ -511,10 +439,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, prepared: PreparedFP8Linea
     training = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
     prepared.validate(weight, training=training and x.requires_grad)
     rows = x if x.ndim == 2 and x.is_contiguous() else x.reshape(-1, x.shape[-1]).contiguous()
-    with on_device(x.device):
-        prepared.wait()
-        if training:
-            y = _FP8Linear.apply(rows, weight, prepared)
-        else:
-            y = _linear_forward(rows, prepared.weight)
+    prepared.wait()
+    held, flipped = prepared.weight, prepared.weight_t
+    y = _lib.binding().fp8_linear(rows, weight, held.data, held.scales, None if flipped is None else flipped.data,
+                                  None if flipped is None else flipped.scales)
     return y if x.ndim == 2 else y.view(*x.shape[:-1], weight.shape[0])

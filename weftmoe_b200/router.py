@@ -7,22 +7,19 @@
 
 The reference leaves the router to its host framework (weftmoe/megatron.py:164-188 takes routes and gates from it);
 the definitions are in include/weftmoe_b200.h beside `wm_router`.  All arithmetic runs in libweftmoe_b200.so; this
-file checks arguments, allocates results and joins the calls to autograd.  Every call enqueues on the current
+file checks arguments, binding/torch_binding.cpp allocates results and joins the calls to autograd.  Every call enqueues on the current
 stream of the logits' device, synchronises nothing and may be captured in a CUDA graph; capture a backward pass
 together with its forward pass (autograd runs a backward pass on the stream of its forward pass).
 """
 from __future__ import annotations
 
-import ctypes
-import functools
 import math
 
 import torch
 
 from . import _lib
-from ._launch import on_device, stream_of
 
-_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+_DTYPES = (torch.bfloat16, torch.float32, torch.float16)
 _SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
@@ -73,162 +70,6 @@ def _require_device(tensor, what):
         raise ValueError(f"{what} must be on a CUDA device")
 
 
-def _rows(logits):
-    """The logits as rows of unit column stride (copied only if they are not)."""
-    tokens, experts = logits.shape
-    plain = (experts == 1 or logits.stride(1) == 1) and (tokens <= 1 or logits.stride(0) >= experts)
-    return logits if plain else logits.contiguous()
-
-
-def _describe(logits, top_k, score, renormalize, scale, bias, padding_mask, sequences):
-    tokens, experts = logits.shape
-    return _lib.WmRouter(
-        logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, _DTYPES[logits.dtype], tokens, experts, top_k,
-        _SCORES[score], int(renormalize), scale, 0 if sequences is None else sequences.shape[0] - 1,
-        None if bias is None else bias.data_ptr(), None if padding_mask is None else padding_mask.data_ptr(),
-        None if sequences is None else sequences.data_ptr())
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(tokens, experts, num_sequences):
-    router = _lib.WmRouter(logits=16, row_stride=experts, dtype=1, tokens=tokens, experts=experts,
-                           num_sequences=num_sequences, sequences=16 if num_sequences else None)
-    size = ctypes.c_int64()
-    _lib.check(_lib.load().wm_router_workspace(ctypes.byref(router), ctypes.byref(size)))
-    return size.value
-
-
-def _loss_buffers(logits, router):
-    """(loss, table, workspace) of a call that computes the loss."""
-    sequences = router.num_sequences
-    return (logits.new_empty((), dtype=torch.float32),
-            logits.new_empty(max(1, sequences) * router.experts + 1, dtype=torch.float32),
-            logits.new_empty(_workspace_bytes(router.tokens, router.experts, sequences), dtype=torch.uint8))
-
-
-def _address(tensor):
-    return None if tensor is None else tensor.data_ptr()
-
-
-def _plain_gradient(gradient):
-    """An incoming gradient as contiguous FP32 (broadcast ones are expanded)."""
-    if gradient is None or (gradient.dtype == torch.float32 and gradient.is_contiguous()):
-        return gradient
-    return gradient.float().contiguous()
-
-
-def _backward(logits, router_args, routes, dgates, table, dloss):
-    if torch.is_grad_enabled():
-        raise RuntimeError("The router's gradients cannot be differentiated again")
-    dgates, dloss = _plain_gradient(dgates), _plain_gradient(dloss)
-    device = logits.device
-    with on_device(device):
-        dlogits = logits.new_empty(logits.shape)
-        router = _describe(logits, *router_args)
-        _lib.check(_lib.load().wm_router_backward(
-            ctypes.byref(router), _address(routes), _address(dgates), _address(table), _address(dloss),
-            dlogits.data_ptr(), stream_of(device, logits, *router_args[-2:], routes, dgates, table, dloss)))
-    return dlogits
-
-
-def _route(logits, top_k, score, renormalize, scale, bias, padding_mask, sequences, balance):
-    """(routes, gates, counts, loss, table); the last three are None without the loss."""
-    device = logits.device
-    tokens, experts = logits.shape
-    with on_device(device):
-        routes = logits.new_empty((tokens, top_k), dtype=torch.int32)
-        gates = logits.new_empty((tokens, top_k), dtype=torch.float32)
-        router = _describe(logits, top_k, score, renormalize, scale, bias, padding_mask, sequences)
-        counts = loss = table = workspace = None
-        if balance:
-            loss, table, workspace = _loss_buffers(logits, router)
-            counts = logits.new_empty((experts,) if sequences is None else (router.num_sequences, experts),
-                                      dtype=torch.int32)
-        _lib.check(_lib.load().wm_router_forward(
-            ctypes.byref(router), routes.data_ptr(), gates.data_ptr(), _address(counts), _address(loss),
-            _address(table), _address(workspace), 0 if workspace is None else workspace.numel(),
-            stream_of(device, logits, bias, padding_mask, sequences)))
-    return routes, gates, counts, loss, table
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_k, score, renormalize, scale, bias, padding_mask):
-        rows = _rows(logits)
-        routes, gates, *_ = _route(rows, top_k, score, renormalize, scale, bias, padding_mask, None, False)
-        ctx.options = (top_k, score, renormalize, scale)
-        ctx.save_for_backward(rows, routes, padding_mask)
-        ctx.mark_non_differentiable(routes)
-        ctx.set_materialize_grads(False)   # no zeros for the routes
-        return routes, gates
-
-    @staticmethod
-    def backward(ctx, _, dgates):
-        if dgates is None:
-            return (None,) * 7
-        rows, routes, padding_mask = ctx.saved_tensors
-        dlogits = _backward(rows, (*ctx.options, None, padding_mask, None), routes,
-                            dgates, None, None)
-        return (dlogits, *[None] * 6)
-
-
-class _RouteAndBalance(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_k, score, renormalize, scale, bias, padding_mask, sequences):
-        rows = _rows(logits)
-        routes, gates, counts, loss, table = _route(rows, top_k, score, renormalize, scale, bias, padding_mask,
-                                                    sequences, True)
-        ctx.options = (top_k, score, renormalize, scale)
-        ctx.save_for_backward(rows, routes, padding_mask, sequences, table)
-        ctx.mark_non_differentiable(routes, counts)
-        ctx.set_materialize_grads(False)
-        return routes, gates, counts, loss
-
-    @staticmethod
-    def backward(ctx, _routes, dgates, _counts, dloss):
-        rows, routes, padding_mask, sequences, table = ctx.saved_tensors
-        if dgates is None and dloss is None:
-            return (None,) * 8
-        if dgates is None:
-            routes = None
-        if dloss is None:
-            table = None
-        dlogits = _backward(rows, (*ctx.options, None, padding_mask, sequences), routes, dgates, table, dloss)
-        return (dlogits, *[None] * 7)
-
-
-class _Balance(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, counts, score, padding_mask, sequences):
-        rows = _rows(logits)
-        loss, table = _balance(rows, counts, score, padding_mask, sequences)
-        ctx.score = score
-        ctx.save_for_backward(rows, padding_mask, sequences, table)
-        return loss
-
-    @staticmethod
-    def backward(ctx, dloss):
-        rows, padding_mask, sequences, table = ctx.saved_tensors
-        dlogits = _backward(rows, (1, ctx.score, False, 1.0, None, padding_mask, sequences), None, None, table,
-                            dloss)
-        return (dlogits, *[None] * 4)
-
-
-def _balance(rows, counts, score, padding_mask, sequences):
-    device = rows.device
-    with on_device(device):
-        router = _describe(rows, 1, score, False, 1.0, None, padding_mask, sequences)
-        loss, table, workspace = _loss_buffers(rows, router)
-        _lib.check(_lib.load().wm_balance_forward(
-            ctypes.byref(router), counts.data_ptr(), loss.data_ptr(), table.data_ptr(), workspace.data_ptr(),
-            workspace.numel(), stream_of(device, rows, counts, padding_mask, sequences)))
-    return loss, table
-
-
-def _wants_gradient(logits):
-    return torch.is_grad_enabled() and logits.requires_grad
-
-
 def route_tokens(logits, top_k, *, score="softmax", renormalize=True, scale=1.0, bias=None, padding_mask=None):
     """Choose top_k experts for every token: (routes int32, gates float32), both [tokens, top_k].
 
@@ -244,9 +85,7 @@ def route_tokens(logits, top_k, *, score="softmax", renormalize=True, scale=1.0,
     _check_vector(bias, "bias", (torch.float32,), logits.shape[1], logits)
     _check_vector(padding_mask, "padding_mask", (torch.bool, torch.uint8), logits.shape[0], logits)
     _require_device(logits, "logits")
-    if not _wants_gradient(logits):
-        return _route(_rows(logits), top_k, score, renormalize, scale, bias, padding_mask, None, False)[:2]
-    return _Route.apply(logits, top_k, score, renormalize, scale, bias, padding_mask)
+    return tuple(_lib.binding().route(logits, top_k, _SCORES[score], renormalize, scale, bias, padding_mask, None, False))
 
 
 def expert_counts(routes, experts, *, sequences=None):
@@ -262,14 +101,7 @@ def expert_counts(routes, experts, *, sequences=None):
         raise ValueError(f"experts must be in [1, {MAX_EXPERTS}]")
     _check_sequences(sequences, routes)
     _require_device(routes, "routes")
-    device = routes.device
-    with on_device(device):
-        counts = routes.new_empty((experts,) if sequences is None else (sequences.shape[0] - 1, experts))
-        _lib.check(_lib.load().wm_expert_counts(
-            routes.data_ptr(), routes.shape[0], routes.shape[1], experts, _address(sequences),
-            0 if sequences is None else sequences.shape[0] - 1, counts.data_ptr(),
-            stream_of(device, routes, sequences)))
-    return counts
+    return _lib.binding().expert_counts(routes, experts, sequences)
 
 
 def balance_loss(logits, counts, *, score="softmax", padding_mask=None, sequences=None):
@@ -288,9 +120,7 @@ def balance_loss(logits, counts, *, score="softmax", padding_mask=None, sequence
             or counts.device != logits.device or not counts.is_contiguous()):
         raise ValueError(f"counts must be a contiguous int32 tensor {list(shape)} on the device of the logits")
     _require_device(logits, "logits")
-    if not _wants_gradient(logits):
-        return _balance(_rows(logits), counts, score, padding_mask, sequences)[0]
-    return _Balance.apply(logits, counts, score, padding_mask, sequences)
+    return _lib.binding().balance(logits, counts, _SCORES[score], padding_mask, sequences)
 
 
 def route_and_balance(logits, top_k, *, score="softmax", renormalize=True, scale=1.0, bias=None, padding_mask=None,
@@ -304,6 +134,5 @@ def route_and_balance(logits, top_k, *, score="softmax", renormalize=True, scale
     _check_vector(padding_mask, "padding_mask", (torch.bool, torch.uint8), logits.shape[0], logits)
     _check_sequences(sequences, logits)
     _require_device(logits, "logits")
-    if not _wants_gradient(logits):
-        return _route(_rows(logits), top_k, score, renormalize, scale, bias, padding_mask, sequences, True)[:4]
-    return _RouteAndBalance.apply(logits, top_k, score, renormalize, scale, bias, padding_mask, sequences)
+    return tuple(_lib.binding().route(logits, top_k, _SCORES[score], renormalize, scale, bias, padding_mask, sequences,
+                                      True))
