@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(256) quantize_both_bf16_kernel(const __nv_bflo
                                                                  unsigned char* __restrict__ qt, float* __restrict__ st) {
   __shared__ uint4 tile[128 * 16];
   __shared__ unsigned tops[4][64];
+  cudaTriggerProgrammaticLaunchCompletion();   // a product behind this may set itself up; it waits before it reads
   const int cblocks = (cols + 127) / 128, rblocks = (rows + 127) / 128;
   const size_t batch = blockIdx.z;
   const int c0 = blockIdx.x * 128, r0 = blockIdx.y * 128;

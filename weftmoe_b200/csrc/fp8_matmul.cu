@@ -698,6 +698,7 @@ pack_scales_kernel(const float* __restrict__ p_scales, int p_rows, int p_shift, 
                    int* __restrict__ findings) {
   __shared__ unsigned char codes[kPackBlocks][128 + 4];
   cudaTriggerProgrammaticLaunchCompletion();   // the product may take its place; it waits for these before it reads
+  cudaGridDependencySynchronize();             // as this kernel does for the one that quantised the operands
   const int p_tiles = (p_rows + 127) / 128;
   const bool of_p = static_cast<int>(blockIdx.x) < p_tiles;
   const int tile = of_p ? blockIdx.x : blockIdx.x - p_tiles;
@@ -874,11 +875,18 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   if (packed) {
     uint8_t* room = static_cast<uint8_t*>(workspace);
     int* findings = reinterpret_cast<int*>(room + packing.findings_at);
-    pack_scales_kernel<<<dim3(packing.p_tiles + packing.q_tiles, packing.parts), 256, 0, stream>>>(
-        as, m, a.p_shift, reinterpret_cast<uint32_t*>(room), bs, n, a.q_shift,
-        reinterpret_cast<uint32_t*>(room + packing.q_at), kblocks, findings);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(packing.p_tiles + packing.q_tiles, packing.parts);
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    WM_CUDA(cudaLaunchKernelEx(&config, pack_scales_kernel, as, m, a.p_shift, reinterpret_cast<uint32_t*>(room), bs, n,
+                               a.q_shift, reinterpret_cast<uint32_t*>(room + packing.q_at), kblocks, findings));
     count_launch();
-    WM_CUDA(cudaGetLastError());
     a.findings = findings;
     a.num_findings = (packing.p_tiles + packing.q_tiles) * packing.parts;
     const uint64_t rows_p = static_cast<uint64_t>(packing.p_tiles) * packing.chunks * 4;
