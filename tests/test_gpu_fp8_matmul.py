@@ -63,7 +63,8 @@ def test_blocks_and_types(m, n, k, a_rows, b_rows, dtype):
 
 @pytest.mark.parametrize("b_rows", (1, 128))
 @pytest.mark.parametrize("m, n, k", [(16, 256, 16384), (64, 2048, 2048), (100, 128, 8192), (1300, 2100, 130),
-                                     (2500, 2900, 300), (1024, 4096, 1152), (4200, 520, 256), (2048, 2048, 2048)])
+                                     (2500, 2900, 300), (1024, 4096, 1152), (4200, 520, 256), (2048, 2048, 2048), (8300, 8200, 250),
+                                     (4100, 4197, 1100)])
 def test_shared_tiles_and_long_grids(m, n, k, b_rows):
     """Tiles whose blocks several CTAs share, and grids of more tiles than there are SMs."""
     check(m, n, k, 1, b_rows)
@@ -71,11 +72,12 @@ def test_shared_tiles_and_long_grids(m, n, k, b_rows):
 
 
 @pytest.mark.parametrize("b_rows", (1, 128))
-@pytest.mark.parametrize("blocks", (1, 7, 8, 9, 31, 32, 33, 65))
+@pytest.mark.parametrize("blocks", (1, 4, 5, 8, 9, 31, 32, 33, 65))
 def test_scales_on_the_tensor_cores(blocks, b_rows):
     """Large tiles with power-of-two scales, up to and beyond one group of 32 blocks and one of the packing kernel;
     a short last block; then the same with one scale that is no power of two, one zero and one NaN."""
-    m, n, k = 1500, 1700, blocks * 128 - 5
+    m, n = (1500, 1700) if blocks > 20 else (4100, 4200)   # large enough for pairs of SMs
+    k = blocks * 128 - 5
     a, b = operand(m, k, 1, 50), operand(n, k, b_rows, 51)
     want = wide(a) @ wide(b).t()
     assert torch.equal(fp8_matmul(a, b, dtype=torch.float32), want.float())
@@ -88,7 +90,7 @@ def test_scales_on_the_tensor_cores(blocks, b_rows):
 
 
 def test_far_powers_of_two_on_the_tensor_cores():
-    a, b = operand(1500, 1100, 1, 52), operand(1700, 1100, 128, 53)
+    a, b = operand(4100, 1100, 1, 52), operand(4200, 1100, 128, 53)
     a.scales[:, 0], b.scales[:, 0] = 2.0 ** 100, 2.0 ** -101
     a.scales[:, 1], b.scales[:, 1] = 2.0 ** -60, 2.0 ** 62
     assert torch.equal(fp8_matmul(a, b, dtype=torch.float32), (wide(a) @ wide(b).t()).float())
@@ -107,7 +109,8 @@ def test_random_products_on_the_tensor_cores(k):
     assert (got - want).norm() <= 2.0 ** -17.5 * want.norm()
 
 
-@pytest.mark.parametrize("m, n, k", [(1, 512, 2048), (33, 700, 1100), (200, 300, 4097), (700, 1300, 2000)])
+@pytest.mark.parametrize("m, n, k", [(1, 512, 2048), (33, 700, 1100), (200, 300, 4097), (700, 1300, 2000),
+                                     (2100, 4100, 2000)])
 @pytest.mark.parametrize("a_rows, b_rows", [(1, 1), (1, 128), (128, 128)])
 def test_any_scales(m, n, k, a_rows, b_rows):
     a, b = operand(m, k, a_rows, 3, "any"), operand(n, k, b_rows, 4, "any")
@@ -152,7 +155,7 @@ def test_empty_sizes():
 
 
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
-@pytest.mark.parametrize("m, n", [(3, 65), (40, 128), (130, 200), (300, 512)])
+@pytest.mark.parametrize("m, n", [(3, 65), (40, 128), (130, 200), (300, 512), (4100, 4200)])
 @pytest.mark.parametrize("left, right", [(8, 8), (1, 2), (0, 3)])
 def test_out_is_a_slice(m, n, left, right, dtype):
     """Rows of a wider tensor, aligned or not: every element beside the slice stays."""
@@ -165,7 +168,7 @@ def test_out_is_a_slice(m, n, left, right, dtype):
     assert (holder == 7).all()
 
 
-@pytest.mark.parametrize("m, n, k", [(9, 200, 512), (200, 300, 512), (600, 1100, 256), (64, 256, 8192)])
+@pytest.mark.parametrize("m, n, k", [(9, 200, 512), (200, 300, 512), (600, 1100, 256), (64, 256, 8192), (4100, 4200, 640)])
 def test_accumulate(m, n, k):
     a, b = operand(m, k, 1, 12), operand(n, k, 1, 13)
     out = torch.randint(-100, 100, (m, n), device="cuda", generator=generator(14)).float()

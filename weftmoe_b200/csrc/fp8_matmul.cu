@@ -743,13 +743,20 @@ Packing packing_of(int m, int n, int kblocks) {
   return k;
 }
 
-// Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  Pairs of SMs take 256 x 256 tiles where
-// those alone fill half of the pairs.
-bool takes_pairs(int m, int n, int sms) {
-  return m > 64 && static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * 4 >= sms;
+// Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  CTA pairs take less time a block and
+// wave but start about 5 us later (the packing kernel, a pair's set-up), so they pay where they save at least 16 blocks
+// of a wave.  One CTA a tile / pairs, us: 1024 x 4096, K = 1024: 10.4 / 12.6, K = 4096: 25.7 / 20.8; 2048 x 4096, K = 1024:
+// 16.9 / 16.3, K = 4096: 46.6 / 31.7; 2048 x 1024, K = 4096: 14.8 / 19.6.
+bool takes_pairs(int m, int n, int kblocks, int sms) {
+  if (m <= 64) return false;
+  const long long single = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128);
+  const long long paired = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256);
+  const long long waves = (single + sms - 1) / sms - (paired + sms / 2 - 1) / (sms / 2);
+  return waves * kblocks >= 16;
 }
-// Packing costs a launch: where K is short the general form is done sooner.
-bool takes_packed(int m, int n, int kblocks, int sms) { return takes_pairs(m, n, sms) && kblocks >= 8; }
+// Packing costs a launch: with very short K the general form is done sooner (8192 x 4096, general / packed, us: K = 256
+// 22.8 / 24.8, K = 512 32.5 / 29.5, and with 1 x 128 blocks on both sides 32.5 / 26.0 and 46.8 / 31.1).
+bool takes_packed(int m, int n, int kblocks, int sms) { return takes_pairs(m, n, kblocks, sms) && kblocks >= 4; }
 
 int sm_count(int* sms) {
   int dev = 0;
@@ -842,7 +849,7 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   const uint64_t pitch = static_cast<uint64_t>(kblocks) * 128;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const bool swap = m <= 64, pairs = takes_pairs(m, n, sms);
+  const bool swap = m <= 64, pairs = takes_pairs(m, n, kblocks, sms);
   const int bn = swap ? (m <= 16 ? 16 : m <= 32 ? 32 : 64) : 128;
   const Packing packing = packing_of(m, n, kblocks);
   const bool packed = workspace && takes_packed(m, n, kblocks, sms);
