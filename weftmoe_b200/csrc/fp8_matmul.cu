@@ -706,15 +706,20 @@ pack_scales_kernel(const float* __restrict__ p_scales, int p_rows, int p_shift, 
   const int rows = of_p ? p_rows : q_rows, shift = of_p ? p_shift : q_shift;
   const int kb0 = blockIdx.y * kPackBlocks, count = min(kPackBlocks, kblocks - kb0);
   int found = 0;
-  for (int i = threadIdx.x; i < 128 * kPackBlocks; i += 256) {
-    const int kb = i % kPackBlocks, r = i / kPackBlocks;
-    unsigned code = 127;
-    if (kb < count && tile * 128 + r < rows) {
-      const unsigned bits = __float_as_uint(__ldg(scales + static_cast<long long>((tile * 128 + r) >> shift) * kblocks + kb0 + kb));
-      code = bits >> 23;   // the biased exponent is the UE8M0 code
-      found |= (bits & 0x7fffffu) != 0 || code == 0 || code >= 255;   // mantissa, zero, infinite, negative
-    }
-    codes[kb][r] = static_cast<unsigned char>(code);
+  constexpr int kEach = 128 * kPackBlocks / 256;
+  const int kb = threadIdx.x % kPackBlocks, r0 = threadIdx.x / kPackBlocks;
+  unsigned bits[kEach];   // all loads before the first use: one after the other they took 10 us
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int row = tile * 128 + r0 + i * (256 / kPackBlocks);
+    bits[i] = kb < count && row < rows
+                  ? __float_as_uint(__ldg(scales + static_cast<long long>(row >> shift) * kblocks + kb0 + kb)) : 0x3f800000u;
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const unsigned code = bits[i] >> 23;   // the biased exponent is the UE8M0 code
+    found |= (bits[i] & 0x7fffffu) != 0 || code == 0 || code >= 255;   // mantissa, zero, infinite, negative
+    codes[kb][r0 + i * (256 / kPackBlocks)] = static_cast<unsigned char>(code);
   }
   found = __syncthreads_or(found);
   if (threadIdx.x == 0) findings[blockIdx.y * gridDim.x + blockIdx.x] = found;
