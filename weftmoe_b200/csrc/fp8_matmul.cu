@@ -749,19 +749,16 @@ Packing packing_of(int m, int n, int kblocks) {
 }
 
 // Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  CTA pairs take less time a block and
-// wave but start about 5 us later (the packing kernel, a pair's set-up), so they pay where they save at least 16 blocks
-// of a wave.  One CTA a tile / pairs, us: 1024 x 4096, K = 1024: 10.4 / 12.6, K = 4096: 25.7 / 20.8; 2048 x 4096, K = 1024:
-// 16.9 / 16.3, K = 4096: 46.6 / 31.7; 2048 x 1024, K = 4096: 14.8 / 19.6.
+// wave but start about 2.6 us later (the packing kernel, a pair's set-up), so they pay where they save at least 8 blocks
+// of a wave.  One CTA a tile / pairs, us: 1024 x 4096, K = 512: 8.0 / 8.7, K = 1024: 10.4 / 10.1, K = 4096: 25.4 / 18.2;
+// 2048 x 4096, K = 512: 12.1 / 10.7, K = 4096: 46.6 / 28.8; 2048 x 1024, K = 4096: 14.9 / 17.2.
 bool takes_pairs(int m, int n, int kblocks, int sms) {
   if (m <= 64) return false;
   const long long single = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128);
   const long long paired = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256);
   const long long waves = (single + sms - 1) / sms - (paired + sms / 2 - 1) / (sms / 2);
-  return waves * kblocks >= 16;
+  return waves * kblocks >= 8;
 }
-// Packing costs a launch: with very short K the general form is done sooner (8192 x 4096, general / packed, us: K = 256
-// 22.8 / 24.8, K = 512 32.5 / 29.5, and with 1 x 128 blocks on both sides 32.5 / 26.0 and 46.8 / 31.1).
-bool takes_packed(int m, int n, int kblocks, int sms) { return takes_pairs(m, n, kblocks, sms) && kblocks >= 4; }
 
 int sm_count(int* sms) {
   int dev = 0;
@@ -857,7 +854,7 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   const bool swap = m <= 64, pairs = takes_pairs(m, n, kblocks, sms);
   const int bn = swap ? (m <= 16 ? 16 : m <= 32 ? 32 : 64) : 128;
   const Packing packing = packing_of(m, n, kblocks);
-  const bool packed = workspace && takes_packed(m, n, kblocks, sms);
+  const bool packed = workspace && pairs;
   if (packed && (workspace_bytes < packing.bytes || reinterpret_cast<uintptr_t>(workspace) % 128)) {
     set_error("wm_fp8_matmul: small or misaligned workspace (wm_fp8_matmul_workspace, 128-byte aligned)");
     return WM_ERR_INVALID;
@@ -956,7 +953,7 @@ extern "C" int wm_fp8_matmul_workspace(int32_t m, int32_t n, int32_t k, int64_t*
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int kblocks = static_cast<int>((static_cast<long long>(k) + 127) / 128);
-  *bytes = takes_packed(m, n, kblocks, sms) ? packing_of(m, n, kblocks).bytes : 0;
+  *bytes = takes_pairs(m, n, kblocks, sms) ? packing_of(m, n, kblocks).bytes : 0;
   return WM_OK;
 }
 
