@@ -71,10 +71,10 @@ __device__ __forceinline__ float reciprocal(float y) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
   return r;
 }
-// 2^t by the exponent unit, two units in the last place; 0 at -inf.
+// 2^t by the exponent unit, two units in the last place; 0 at -inf and below 2^-126.
 __device__ __forceinline__ float power_of_2(float t) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(t));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
 // Exponentials are powers of 2 of x log2 e.  exp(x - top) is 2^(x log2 e - c) with c the rounded top log2 e: the
@@ -661,27 +661,37 @@ router_backward_kernel(const Rows a, const int* __restrict__ routes, const float
   const int end = static_cast<int>(min(from + a.chunk, static_cast<long long>(a.tokens)));
   int b = 0, b_end = -1;
   RowPieces<T, V, VEC> next;
-  if (from < end) fetch_row<T, V, VEC>(a, from, lane, next);
+  int next_expert = -1;
+  float next_g = 0.0f;
+  const auto fetch_choice = [&](int row) {
+    if (routes == nullptr || lane >= a.top_k) return;
+    const long long at = static_cast<long long>(row) * a.top_k + lane;
+    next_expert = routes[at];
+    next_g = dgates[at];
+  };
+  if (from < end) {
+    fetch_row<T, V, VEC>(a, from, lane, next);
+    fetch_choice(static_cast<int>(from));
+  }
   for (int row = static_cast<int>(min(from, static_cast<long long>(a.tokens))); row < end; ++row) {
     if (row >= b_end) {
       b = sequence_of(a, row);
       b_end = max(row + 1, sequence_end(a, b));
     }
     const RowPieces<T, V, VEC> here = next;
-    if (row + 1 < end) fetch_row<T, V, VEC>(a, row + 1, lane, next);
+    int expert = next_expert;
+    float g = a.scale * next_g;
+    if (row + 1 < end) {
+      fetch_row<T, V, VEC>(a, row + 1, lane, next);
+      fetch_choice(row + 1);
+    }
     float d[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.0f;
     if (row_live(a, row, b)) {
-      int expert = -1;
-      float logit = 0.0f, g = 0.0f;
-      if (routes != nullptr && lane < a.top_k) {
-        const long long at = static_cast<long long>(row) * a.top_k + lane;
-        expert = routes[at];
-        if (static_cast<unsigned>(expert) >= static_cast<unsigned>(a.experts)) expert = -1;
-        g = a.scale * dgates[at];
-        if (expert >= 0) logit = as_float((static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.stride)[expert]);
-      }
+      float logit = 0.0f;
+      if (static_cast<unsigned>(expert) >= static_cast<unsigned>(a.experts)) expert = -1;
+      if (expert >= 0) logit = as_float((static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.stride)[expert]);
       float x[V], h[V], rest[V];
       unpack_row<T, V, VEC>(a, lane, here, x);
       const RowTop r = row_top<V>(x, a.sigmoid);
@@ -691,7 +701,7 @@ router_backward_kernel(const Rows a, const int* __restrict__ routes, const float
       } else if (r.any) {
         float sum = 1.0f;
         if (shares) sum = row_shares<V>(x, a.sigmoid, r.top, h, rest);
-        const float inv = 1.0f / sum;
+        const float inv = reciprocal(sum);
         if (table != nullptr) {
           const float* q = table + static_cast<long long>(b) * a.experts;
           float mean = 0.0f;
