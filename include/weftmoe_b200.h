@@ -343,15 +343,16 @@ typedef struct wm_router {
 /* Bytes of the workspace of a forward call that computes the loss. */
 WM_API int wm_router_workspace(const wm_router* router, int64_t* bytes);
 /* routes / gates [tokens][top_k].  counts, loss, table and workspace are NULL together (no loss), or:
- * counts [max(1, num_sequences)][experts], loss [1], table [max(1, num_sequences) * experts + 1] FP32, which the
- * backward call reads.  The workspace is free again when the call's kernels are done. */
+ * counts [max(1, num_sequences)][experts], loss [1], table [max(1, num_sequences) * experts + 1] FP32 (16-byte
+ * aligned), which the backward call reads.  The workspace is free again when the call's kernels are done. */
 WM_API int wm_router_forward(const wm_router* router, int32_t* routes, float* gates, int32_t* counts, float* loss,
                              float* table, void* workspace, int64_t workspace_bytes, void* stream);
 /* The loss for given counts (another router's, or summed over ranks). */
 WM_API int wm_balance_forward(const wm_router* router, const int32_t* counts, float* loss, float* table,
                               void* workspace, int64_t workspace_bytes, void* stream);
 /* dlogits [tokens][experts] contiguous, of the logits' type: the gates' part (routes, dgates [tokens][top_k]), the
- * loss's part (table, dloss [1] on the device), or both added in FP32; the absent pair is NULL. */
+ * loss's part (table, dloss [1] on the device), or both added in FP32; the absent pair is NULL.  routes:
+ * those of the forward call (no id twice in a row, -1 = no route). */
 WM_API int wm_router_backward(const wm_router* router, const int32_t* routes, const float* dgates,
                               const float* table, const float* dloss, void* dlogits, void* stream);
 /* counts [max(1, num_sequences)][experts] = routes per expert; ids outside [0, experts) count nowhere. */

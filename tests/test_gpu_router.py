@@ -89,6 +89,23 @@ def test_bias_selects_but_does_not_weigh(score, experts, spread):
     check_route(make(37, experts), 6, vector(37 * 6, 2).view(37, 6), score=score, bias=vector(experts, 3, spread))
 
 
+@pytest.mark.parametrize("value", (torch.finfo(torch.float32).min, -1e10, torch.finfo(torch.float32).max))
+@pytest.mark.parametrize("score", ("softmax", "sigmoid"))
+@pytest.mark.parametrize("experts, left", [(8, 2), (8, 5), (31, 3), (64, 4), (300, 6)])
+def test_bias_of_the_lowest_value_puts_experts_last(experts, left, score, value):
+    """All but `left` experts are banned (or, by the largest value, put first); top_k reaches into the others, and two
+    that are left are closer than 32 bits tell."""
+    bias = torch.full((experts,), value)
+    keep = torch.arange(left) * (experts // left)
+    bias[keep] = 0.0
+    logits = make(21, experts, seed=17)
+    logits[:, keep[1]] = logits[:, keep[0]] * (1 + 2 ** -22)
+    logits[3, keep] = -float("inf")                              # none of them left
+    logits[4, experts // 2:] = -float("inf")
+    for top_k in (left, min(left + 2, experts)):
+        check_route(logits, top_k, vector(21 * top_k, 18).view(21, top_k), bias=bias, score=score)
+
+
 @pytest.mark.parametrize("bias", (None, torch.zeros(64)))
 def test_ties_go_to_the_lowest_expert(bias):
     logits = torch.randint(-2, 3, (50, 64), generator=torch.Generator().manual_seed(4)).float()
@@ -408,3 +425,11 @@ def test_long_batches_pass_32_bits():
     want = reference(tail, 2, dgates=dgates[-64:].cpu())
     gradient_close(dx[-64:], want, tail)
     assert not dx[:1000].any()
+
+
+@pytest.mark.parametrize("sequences", (1, 32, 33, 500))
+def test_counts_of_no_tokens(sequences):
+    routes = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    offsets = torch.zeros(sequences + 1, dtype=torch.int32, device="cuda")
+    counts = expert_counts(routes, 5, sequences=offsets)
+    assert counts.shape == (sequences, 5) and not counts.any()

@@ -107,6 +107,24 @@ def test_c_entries_refuse_before_any_device_work():
         assert lib.wm_router_backward(ctypes.byref(r), 64, 64, None, None, 64, None) == _lib.WM_ERR_INVALID
     for pair in ((64, None, None, None), (None, None, 64, None), (None, None, None, None)):
         assert lib.wm_router_backward(ctypes.byref(good), *pair, 64, None) == _lib.WM_ERR_INVALID
+    # addresses that are not multiples of their elements (the table's: of 16 bytes)
+    for change in (dict(logits=66), dict(logits=65, dtype=0), dict(logits=65, dtype=2), dict(bias=66),
+                   dict(sequences=66, num_sequences=1)):
+        r = _description(**change)
+        assert lib.wm_router_workspace(ctypes.byref(r), ctypes.byref(size)) == _lib.WM_ERR_INVALID, change
+        assert lib.wm_router_backward(ctypes.byref(r), 64, 64, None, None, 64, None) == _lib.WM_ERR_INVALID, change
+    for outputs in ((66, 64, None, None, None, None, 0), (64, 65, None, None, None, None, 0),
+                    (64, 64, 66, 64, 64, 64, size.value), (64, 64, 64, 65, 64, 64, size.value),
+                    (64, 64, 64, 64, 66, 64, size.value)):
+        assert lib.wm_router_forward(ctypes.byref(good), *outputs, None) == _lib.WM_ERR_INVALID, outputs
+    for given in ((66, 64, 64), (64, 66, 64), (64, 64, 66)):
+        assert lib.wm_balance_forward(ctypes.byref(good), *given, 64, size.value, None) == _lib.WM_ERR_INVALID, given
+    for pairs in ((66, 64, None, None, 64), (64, 66, None, None, 64), (None, None, 68, 64, 64), (None, None, 64, 66, 64),
+                  (64, 64, None, None, 66)):
+        assert lib.wm_router_backward(ctypes.byref(good), *pairs, None) == _lib.WM_ERR_INVALID, pairs
+    for routes, sequences, counts in ((66, None, 64), (64, 66, 64), (64, None, 65)):
+        assert lib.wm_expert_counts(routes, 4, 2, 8, sequences, int(sequences is not None), counts,
+                                    None) == _lib.WM_ERR_INVALID
     assert lib.wm_expert_counts(64, 4, 33, 8, None, 0, 64, None) == _lib.WM_ERR_INVALID
     assert lib.wm_expert_counts(None, 4, 2, 8, None, 0, 64, None) == _lib.WM_ERR_INVALID
 

@@ -291,11 +291,11 @@ __device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, 
 }
 
 // The K largest (value, lowest expert first) of the warp's V x 32 values, `most` the lane's largest; -inf is no
-// candidate.  The (K+1)th largest of the lanes' maxima is at most the (K+1)th largest value, so the values from it up hold the choice and the one
-// behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They, and with a margin what is at
-// most so much smaller, are gathered in `held` (32 of this warp), and each counts the ones before it.  Lane k gets choice
-// k and its value; `behind` the next value (-inf: none).  Returns the number of candidates, which stay in `held` in
-// their order; above 32 (many equal values) nothing is chosen.
+// candidate.  The (K+1)th largest of the lanes' maxima is at most the (K+1)th largest value, so the values from it up
+// hold the choice and the one behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They,
+// and with a margin what is at most so much smaller, are gathered in `held` (32 of this warp), and each counts the ones
+// before it.  Lane k gets choice k and its value; `behind` the next value (-inf: none).  Returns the number of
+// candidates, which stay in `held` in their order; above 32 (many equal values) nothing is chosen.
 template <int V, int VEC>
 __device__ __forceinline__ int choose(const float (&x)[V], float most, float margin, int top_k, int lane, float2* held, int& expert,
                                       float& its, float& behind) {
@@ -306,7 +306,7 @@ __device__ __forceinline__ int choose(const float (&x)[V], float most, float mar
     if (key == border) key = 0;
   }
   float from = -FLT_MAX;
-  if (border != 0) from = unordered(border) - margin * (1.0f + fabsf(unordered(border)));
+  if (border != 0) from = fmaxf(from, unordered(border) - margin * (1.0f + fabsf(unordered(border))));   // never -inf
   int mine = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) mine += x[j] >= from;
@@ -846,6 +846,12 @@ Plan plan_of(const wm_router& r) {
   return p;
 }
 
+// Addresses that are multiples of `bytes` (null is one).
+template <class... P>
+bool aligned(uintptr_t bytes, P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0;
+}
+
 int check_rows(const char* what, const wm_router* r) {
   if (!r) { set_error("%s: null arguments", what); return WM_ERR_INVALID; }
   if (r->tokens < 0 || r->tokens > kMaxTokens || r->experts < 1 || r->experts > kMaxExperts || r->dtype < 0 || r->dtype > 2 ||
@@ -853,6 +859,10 @@ int check_rows(const char* what, const wm_router* r) {
       (r->sequences ? r->num_sequences < 1 : r->num_sequences != 0) || r->num_sequences > 65535) {
     set_error("%s: logits must be [fewer than 2^26 tokens][experts] BF16 / FP32 / FP16 rows of 1..%d experts, score 0 (softmax) "
               "or 1 (sigmoid), 1..65535 sequences with their offsets", what, kMaxExperts);
+    return WM_ERR_INVALID;
+  }
+  if (!aligned(r->dtype == 1 ? 4 : 2, r->logits) || !aligned(4, r->bias, r->sequences)) {
+    set_error("%s: logits, bias or sequences not aligned to their elements", what);
     return WM_ERR_INVALID;
   }
   return WM_OK;
@@ -952,10 +962,10 @@ extern "C" int wm_router_forward(const wm_router* r, int32_t* routes, float* gat
   if (int rc = check_choice("wm_router_forward", r)) return rc;
   const Plan p = plan_of(*r);
   const bool balance = counts || loss || table || workspace;
-  if ((r->tokens > 0 && (!routes || !gates)) ||
+  if ((r->tokens > 0 && (!routes || !gates)) || !aligned(4, routes, gates, counts, loss, table) ||
       (balance && (!counts || !loss || !table || !workspace || workspace_bytes < p.bytes ||
                    reinterpret_cast<uintptr_t>(workspace) % 16))) {
-    set_error("wm_router_forward: null output, or a missing or small workspace (wm_router_workspace, 16-byte aligned)");
+    set_error("wm_router_forward: null or misaligned output, or a missing or small workspace (wm_router_workspace, 16-byte aligned)");
     return WM_ERR_INVALID;
   }
   if (r->tokens == 0 && !balance) return WM_OK;
@@ -973,9 +983,9 @@ extern "C" int wm_balance_forward(const wm_router* r, const int32_t* counts, flo
                                   void* workspace, int64_t workspace_bytes, void* stream_) {
   if (int rc = check_rows("wm_balance_forward", r)) return rc;
   const Plan p = plan_of(*r);
-  if (!counts || !loss || !table || !workspace || workspace_bytes < p.bytes ||
+  if (!counts || !loss || !table || !aligned(4, counts, loss, table) || !workspace || workspace_bytes < p.bytes ||
       reinterpret_cast<uintptr_t>(workspace) % 16) {
-    set_error("wm_balance_forward: null argument, or a small workspace (wm_router_workspace, 16-byte aligned)");
+    set_error("wm_balance_forward: null or misaligned argument, or a small workspace (wm_router_workspace, 16-byte aligned)");
     return WM_ERR_INVALID;
   }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -1000,6 +1010,10 @@ extern "C" int wm_router_backward(const wm_router* r, const int32_t* routes, con
     set_error("wm_router_backward: routes go with dgates, table with dloss; one pair and dlogits are needed");
     return WM_ERR_INVALID;
   }
+  if (!aligned(4, routes, dgates, dloss) || !aligned(16, table) || !aligned(r->dtype == 1 ? 4 : 2, dlogits)) {
+    set_error("wm_router_backward: misaligned argument (table: 16 bytes, the others to their elements)");
+    return WM_ERR_INVALID;
+  }
   if (r->tokens == 0) return WM_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const Rows a = rows_of(*r, plan_of(*r));
@@ -1012,7 +1026,8 @@ extern "C" int wm_router_backward(const wm_router* r, const int32_t* routes, con
 extern "C" int wm_expert_counts(const int32_t* routes, int32_t tokens, int32_t top_k, int32_t experts,
                                 const int32_t* sequences, int32_t num_sequences, int32_t* counts, void* stream_) {
   if (tokens < 0 || tokens > kMaxTokens || top_k < 1 || top_k > 32 || experts < 1 || experts > kMaxExperts || !counts ||
-      (tokens > 0 && !routes) || (sequences ? num_sequences < 1 : num_sequences != 0) || num_sequences > 65535) {
+      (tokens > 0 && !routes) || (sequences ? num_sequences < 1 : num_sequences != 0) || num_sequences > 65535 ||
+      !aligned(4, routes, sequences, counts)) {
     set_error("wm_expert_counts: routes [fewer than 2^26 tokens][1..32], 1..%d experts, 1..65535 sequences with their offsets",
               kMaxExperts);
     return WM_ERR_INVALID;
@@ -1032,6 +1047,7 @@ extern "C" int wm_expert_counts(const int32_t* routes, int32_t tokens, int32_t t
     return WM_OK;
   }
   WM_CUDA(cudaMemsetAsync(counts, 0, static_cast<size_t>(rows) * experts * 4, stream));
+  if (tokens == 0) return WM_OK;
   const int want = (tokens + 127) / 128;
   const int blocks = want < 296 ? want : 296;
   a.chunk = (tokens + blocks - 1) / blocks;

@@ -75,7 +75,7 @@ def route_tokens(logits, top_k, *, score="softmax", renormalize=True, scale=1.0,
 
     score        "softmax" over the token's experts, or "sigmoid" of each.
     renormalize  divide the chosen scores by their sum; `scale` multiplies the gates.
-    bias         float32 [experts], added to the scores for the choice only (gates and gradients do not see it).
+    bias         finite float32 [experts], added to the scores for the choice only (gates and gradients do not see it).
     padding_mask bool [tokens], True = padding: routes -1, gates 0, no gradient.
     A logit of -inf takes the expert out for that token; where fewer than top_k are left the rest are -1 with gate 0.
     Ties go to the lowest expert.  Gates are differentiable by the logits."""
