@@ -7,6 +7,7 @@ S the sum of the terms' magnitudes: a block's 128 products are exact, their FP32
 import pytest
 import torch
 
+from weftmoe_b200 import _lib
 from weftmoe_b200.fp8 import (FP8Tensor, _quantize_fp8_both, fp8_linear, fp8_matmul, poll_fp8_matmul,
                               prepare_fp8_linear, quantize_fp8)
 
@@ -166,6 +167,26 @@ def test_out_is_a_slice(m, n, left, right, dtype):
     assert torch.equal(view, (wide(a) @ wide(b).t()).float().to(dtype))
     view.fill_(7.0)
     assert (holder == 7).all()
+
+
+def test_a_written_out_is_a_change_in_place():
+    a, b = operand(9, 128, 1, 3), operand(40, 128, 128, 4)
+    out = torch.zeros(9, 40, device="cuda")
+    leaf = torch.ones(9, 40, device="cuda", requires_grad=True)
+    product = leaf * out                                          # keeps out for its gradient
+    fp8_matmul(a, b, dtype=torch.float32, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        out = torch.zeros(9, 40, device="cuda")
+        assert torch.equal(fp8_matmul(a, b, dtype=torch.float32, out=out), fp8_matmul(a, b, dtype=torch.float32))
+
+
+def test_linear_entry_of_an_empty_sum():
+    out = torch.full((5, 8), 7.0, device="cuda", dtype=torch.bfloat16)
+    code = _lib.load().wm_fp8_linear(None, 0, 5, 0, None, None, 8, out.data_ptr(), None, 0,
+                                     torch.cuda.current_stream().cuda_stream)
+    assert code == _lib.WM_OK and not out.any()
 
 
 @pytest.mark.parametrize("m, n, k", [(9, 200, 512), (200, 300, 512), (600, 1100, 256), (64, 256, 8192), (4100, 4200, 640)])

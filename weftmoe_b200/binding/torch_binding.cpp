@@ -265,6 +265,7 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& as, int64_t a_block_rows, const
   Tensor out = given.has_value() ? *given : at::empty({m, n}, as.options().dtype(out_is_f32 ? at::kFloat : at::kBFloat16));
   matmul_into(launch, a, as, a_block_rows, b, bs, b_block_rows, out, m > 1 ? out.stride(0) : std::max<int64_t>(n, 1), m, n,
               k, accumulate);
+  if (given.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
   return out;
 }
 

@@ -927,7 +927,7 @@ extern "C" int wm_fp8_linear(const void* x, int32_t x_is_f32, int32_t rows, int3
   const long long rest_at = (scales_at + static_cast<long long>(rows) * kblocks * 4 + 127) / 128 * 128;
   int64_t rest = 0;
   if (int rc = wm_fp8_matmul_workspace(rows, n, k, &rest)) return rc;
-  if (!workspace || workspace_bytes < rest_at + rest || reinterpret_cast<uintptr_t>(workspace) % 128) {
+  if ((!workspace && rest_at + rest > 0) || workspace_bytes < rest_at + rest || reinterpret_cast<uintptr_t>(workspace) % 128) {
     set_error("wm_fp8_linear: missing, small or misaligned workspace (wm_fp8_linear_workspace, 128-byte aligned)");
     return WM_ERR_INVALID;
   }

@@ -195,7 +195,7 @@ def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.T
     """A @ B^T of A [M, K] and B [N, K], blocks of 1 or 128 rows on either side, any scales.
 
     Enqueues on the current stream and returns; may be captured.  `out` (BF16 or FP32 like `dtype`) may be a
-    slice of a wider tensor: unit column stride, rows at least N apart.  `accumulate` adds into an FP32 `out`."""
+    slice of a wider tensor: unit column stride, rows at least N apart; writing it counts as a change in place.  `accumulate` adds into an FP32 `out`."""
     if not isinstance(a, FP8Tensor) or not isinstance(b, FP8Tensor):
         raise TypeError("fp8_matmul takes FP8Tensor operands")
     if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[1] or a.data.device != b.data.device:
