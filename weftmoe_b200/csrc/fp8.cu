@@ -188,8 +188,9 @@ __device__ __forceinline__ unsigned codes_of(unsigned a, unsigned b) {
 
 // 1 x 128 blocks of BF16 x along its columns (q, s) and along its rows (qt, st: the blocks of x^T), either of
 // them optional, from one read.  HBM-bound: 2 + 1 + 1 bytes an element.  One CTA per 128 x 128 tile.  WIDE: cols % 8 == 0
-// and 16-byte aligned rows, read 16 bytes at a time; otherwise element by element.  A row's block lies in 16 lanes and is quantised in registers; for the columns the tile passes
-// through shared memory, and a thread takes two columns of 32 rows, so that it writes whole 32-byte sectors of qt.
+// and 16-byte aligned rows, read 16 bytes at a time; otherwise element by element.  A row's block lies in 16 lanes and is
+// quantised in registers; for the columns the tile passes through shared memory, and a thread takes two columns of 32
+// rows, so that it writes whole 32-byte sectors of qt.
 // Magnitudes are compared as their bit patterns, in which infinities and NaN come out on top.
 // 8192 x 4096, both: 33 us, 4.1 TB/s (a copy of as many bytes: 22 us); two passes over x took 200 us.
 template <bool WIDE>

@@ -18,11 +18,20 @@
 // so a byte of either operand feeds twice the arithmetic of a 128 x 128 tile.
 // PAIR, scales all powers of two (what this library's quantisers give): the tensor cores apply the scales themselves
 // (kind::mxf8f6f4.block_scale, scales as UE8M0 in TMEM) and accumulate up to 32 blocks before the adding warps take them
-// over.  The accumulator cuts what it cannot hold, so its error grows with the number of blocks (4.9e-7 of the result at
-// K = 8192, 3.0e-6 at 32768, against 1.3e-7 of FP32 sums of products); 32 blocks keep it below 3e-7.  A kernel in front packs the
-// scales and notes whether one is no power of two; the product then takes the general form above.
+// over.  The accumulator cuts what it cannot hold, so its error grows with the number of blocks (normal operands: 4.9e-7
+// of the result at K = 8192 and 3.0e-6 at 32768 in one go); with 32 it stays at 2.2e-7 from K = 4096 up (general form: 0.7
+// to 2.3e-7 from 4096 to 32768), and at 1.4e-6 where all products are positive and every cut goes the same way (general
+// form 0.9 to 2.5e-7).  E4M3 itself is off by up to 2^-4 an operand.  A kernel in front packs the scales and notes
+// whether one is no power of two; the product then takes the general form above.
 // Otherwise `split` CTAs of a cluster may share one tile, each a range of the blocks; their sums are joined through
 // distributed shared memory in a fixed order.
+//
+// What bounds it.  Few rows (64 x 4096 x 4096: 11.5 us; its 17 MB of weights take 2.7 us to read): the start of the
+// kernel, 8 blocks a CTA one after the other, and the join of four sums.  Large products with packed scales (8192 x
+// 4096 x 4096: 97 us, 2.8 PFLOP/s, tensor pipe 76 % busy): operands from shared memory and L2; repeated for seconds
+// the power limit makes it 116 us.  Long K on few tiles (4096 x 2048, K = 8190: 57 us, 60 % busy): 128 tiles on 74 pairs,
+// a second wave that is three quarters full.  General scales on pairs (147 and 154 us for these two): the adding warps, 128
+// accumulators a thread read, scaled and added for every block.
 #include "../../include/weftmoe_b200.h"
 #include "gemm.cuh"
 #include "kernels.h"
@@ -196,7 +205,7 @@ struct Matmul {
   static_assert(PAIR || BN * 128 * 4 <= kStages * kStageBytes, "the joined sums fit in the stages");
   // PAIR with packed scales: chunks of 128 rows' scales of four blocks, one of P and two of Q, come with every fourth
   // stage, in place of the table; in TMEM twice behind the one accumulator, 16 columns each.  (A chunk for every block, the
-  // same byte four times, took 131 us for 8192 x 4096 x 4096 where four blocks a chunk take 117.)
+  // same byte four times, took 131 us for 8192 x 4096 x 4096 where four blocks a chunk took 117, repeated without a pause.)
   static constexpr int kPackedBytes = 3 * 512;
   static constexpr uint32_t kTmemScales = BN;
   static_assert(!PAIR || kStages * kPackedBytes <= kScaleBytes, "packed scales fit where the table is");
@@ -691,7 +700,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
 }
 
 // FP32 scales -> UE8M0 chunks [ceil(rows / 128)][ceil(kblocks / 4)][512 bytes] in the 4 x 32 order of tcgen05.cp (word
-// (r % 32) * 4 + r / 32 holds row r, byte i the block 4 c + i), of P and then of Q.  Rows and blocks behind the last get scale 1.  Each CTA, one of 128 rows x 32 blocks, notes whether it met a scale that is no power of two.
+// (r % 32) * 4 + r / 32 holds row r, byte i the block 4 c + i), of P and then of Q.  Rows and blocks behind the last get
+// scale 1.  Each CTA, one of 128 rows x 32 blocks, notes whether it met a scale that is no power of two.  5.5 us alone,
+// nearly all of it latency (1 MB in, 0.3 MB out for 8192 x 4096 scaled by rows); behind a quantiser its start is hidden.
 __global__ void __launch_bounds__(256)
 pack_scales_kernel(const float* __restrict__ p_scales, int p_rows, int p_shift, uint32_t* __restrict__ p_out,
                    const float* __restrict__ q_scales, int q_rows, int q_shift, uint32_t* __restrict__ q_out, int kblocks,
