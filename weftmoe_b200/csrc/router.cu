@@ -32,6 +32,9 @@ constexpr int kFinishWarps = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTokens = (1 << 26) - 1;   // x 32 routes: counts fit in 32 bits
 constexpr int kMaxBlocks = 1184;  // 148 SMs x 8
+constexpr int kFewChoices = 12;     // see choose
+template <bool MANY>
+constexpr int kCandidates = MANY ? 64 : 32;   // of one row, for its choice
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ float as_float(float v) { return v; }
@@ -227,7 +230,7 @@ __device__ __forceinline__ float row_shares(const float (&x)[V], bool sigmoid, f
 }
 
 // The choice of one row from memory, in K rounds over all experts, by 64-bit scores: for rows with too many candidates
-// (more than 32 equal values).  Out of line and without arrays it costs the other rows no registers.
+// (some 64 equal values).  Out of line and without arrays it costs the other rows no registers.
 template <class T>
 __device__ __noinline__ int choose_slowly(const T* logits, int experts, int top_k, const float* bias, bool sigmoid,
                                           float top, int lane) {
@@ -261,8 +264,8 @@ __device__ __noinline__ int choose_slowly(const T* logits, int experts, int top_
   return expert;
 }
 
-// The n <= 32 candidates in `held` (any order), ranked by their 64-bit scores; lane k gets choice k.  A lane takes one
-// candidate, so this costs one exponential in 64 bits (and for softmax the row's sum).
+// The n <= 64 candidates in `held` (any order), ranked by their 64-bit scores; lane k gets choice k.  A lane takes one
+// candidate or two, so this costs one exponential in 64 bits or two (and for softmax the row's sum).
 template <class T>
 __device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, const float* bias, bool sigmoid,
                                        float top, int lane, float2* held, int n) {
@@ -273,64 +276,32 @@ __device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, 
     for (int e = lane; e < experts; e += 32) sum += exp(static_cast<double>(as_float(logits[e])) - top);
     sum = warp_sum(sum);
   }
-  int expert = 0x7fffffff;
-  double v = -INFINITY;
-  if (lane < n) {
-    expert = __float_as_int(held[lane].y);
-    const double x = as_float(logits[expert]);
-    v = (sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum) + static_cast<double>(__ldg(bias + expert));
+  int expert[2] = {0x7fffffff, 0x7fffffff}, before[2] = {0, 0};
+  double v[2] = {-INFINITY, -INFINITY};
+  for (int c = 0; c < 2; ++c) {
+    if (lane + 32 * c >= n) break;
+    expert[c] = __float_as_int(held[lane + 32 * c].y);
+    const double x = as_float(logits[expert[c]]);
+    v[c] = (sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum) + static_cast<double>(__ldg(bias + expert[c]));
   }
-  int before = 0;
   for (int i = 0; i < n; ++i) {
-    const double w = __shfl_sync(kAll, v, i);
-    const int e = __shfl_sync(kAll, expert, i);
-    before += w > v || (w == v && e < expert);
+    const double w = __shfl_sync(kAll, i < 32 ? v[0] : v[1], i & 31);
+    const int e = __shfl_sync(kAll, i < 32 ? expert[0] : expert[1], i & 31);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) before[c] += w > v[c] || (w == v[c] && e < expert[c]);
   }
   __syncwarp();
-  if (lane < n) held[before].y = __int_as_float(expert);
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (lane + 32 * c < n) held[before[c]].y = __int_as_float(expert[c]);
   __syncwarp();
-  expert = lane < min(n, top_k) ? __float_as_int(held[lane].y) : -1;
+  const int chosen = lane < min(n, top_k) ? __float_as_int(held[lane].y) : -1;
   __syncwarp();
-  return expert;
+  return chosen;
 }
 
-// The K largest (value, lowest expert first) of the warp's V x 32 values, `most` the lane's largest; -inf is no
-// candidate.  The (K+1)th largest of the lanes' maxima is at most the (K+1)th largest value, so the values from it up
-// hold the choice and the one behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They,
-// and with a margin what is at most so much smaller, are gathered in `held` (32 of this warp), and each counts the ones
-// before it.  Lane k gets choice k and its value; `behind` the next value (-inf: none).  Returns the number of
-// candidates, which stay in `held` in their order; above 32 (many equal values) nothing is chosen.
-template <int V, int VEC>
-__device__ __forceinline__ int choose(const float (&x)[V], float most, float margin, int top_k, int lane, float2* held, int& expert,
-                                      float& its, float& behind) {
-  unsigned key = most > -INFINITY ? ordered(most) : 0u, border = 0;
-  for (int k = 0; k <= top_k; ++k) {   // equal maxima go at once: the border is then lower, which is as good
-    border = __reduce_max_sync(kAll, key);
-    if (border == 0) break;
-    if (key == border) key = 0;
-  }
-  float from = -FLT_MAX;
-  if (border != 0) from = fmaxf(from, unordered(border) - margin * (1.0f + fabsf(unordered(border))));   // never -inf
-  int mine = 0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) mine += x[j] >= from;
-  // places: lanes before this one with at least 1, 2, ... candidates
-  int at = 0, n = 0;
-  const unsigned before_me = (1u << lane) - 1;
-  for (int c = 1;; ++c) {
-    const unsigned lanes = __ballot_sync(kAll, mine >= c);
-    if (lanes == 0) break;
-    at += __popc(lanes & before_me);
-    n += __popc(lanes);
-  }
-  if (n > 32) return n;
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (x[j] >= from) held[at++] = make_float2(x[j], __int_as_float(expert_of<VEC>(j, lane)));
-  __syncwarp();
-  if (lane >= n) held[lane] = make_float2(-INFINITY, __int_as_float(0x7fffffff));   // ranks behind all candidates
-  __syncwarp();
-  const float2 me = held[lane];
+// How many of the first n candidates (n rounded up to four; those behind are last) come before this one.
+__device__ __forceinline__ int before_of(const float2& me, const float2* held, int n) {
   int before = 0;
   for (int i = 0; i < n; i += 4) {
 #pragma unroll
@@ -338,6 +309,95 @@ __device__ __forceinline__ int choose(const float (&x)[V], float most, float mar
       const float2 other = held[i + w];
       before += other.x > me.x || (other.x == me.x && __float_as_int(other.y) < __float_as_int(me.y));
     }
+  }
+  return before;
+}
+template <int V>
+__device__ __forceinline__ int count_from(const float (&x)[V], float from) {
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mine += x[j] >= from;
+  return __reduce_add_sync(kAll, mine);
+}
+// A higher border for a row with more than 64 values from `border` up: one with more than top_k of them, and
+// few enough, by halving the words between it and `top`.  Unchanged where equal values leave none.
+template <int V>
+__device__ __forceinline__ float closer_border(const float (&x)[V], float border, float top, int top_k) {
+  unsigned low = ordered(border), high = ordered(top) + 1;
+  while (high - low > 1) {
+    const unsigned middle = low + (high - low) / 2;
+    const int n = count_from<V>(x, unordered(middle));
+    if (n <= top_k) high = middle;
+    else if (n > kCandidates<true> - 4) low = middle;   // a few places are left for the margin
+    else return unordered(middle);
+  }
+  return border;
+}
+
+// The K largest (value, lowest expert first) of the warp's V x 32 values, `most` the lane's largest; -inf is no
+// candidate.  The (K+1)th largest of the lanes' maxima is at most the (K+1)th largest value, so the values from it up
+// hold the choice and the one behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They,
+// and with a margin what is at most so much smaller, are gathered in `held` (kCandidates of this warp), and each counts the ones
+// before it.  Lane k gets choice k and its value; `behind` the next value (-inf: none).  Returns the number of
+// candidates, which stay in `held` in their order; above kCandidates (many equal values) nothing is chosen.
+// MANY: for K above kFewChoices the border of 32 lanes leaves more candidates (24 on average at K = 16, all values at
+// K = 32): room for 64, two a lane, and a border moved up by halving.  65536 x 512 BF16 by logits, with / without: K = 8
+// 80 / 76 us, K = 16 116 / 329, K = 32 202 / 1959; up to 12 the 32 places overflow in less than one row of 10000.
+template <bool MANY, int V, int VEC>
+__device__ __forceinline__ int choose(const float (&x)[V], float most, float margin, int top_k, int lane, float2* held, int& expert,
+                                      float& its, float& behind) {
+  unsigned key = most > -INFINITY ? ordered(most) : 0u, top = 0, border = 0;
+  for (int k = 0; k <= top_k; ++k) {   // equal maxima go at once: the border is then lower, which is as good
+    const unsigned next = __reduce_max_sync(kAll, key);
+    if (k == 0) top = next;
+    if (next == 0) {   // fewer lanes: the least of their maxima may do, or else all values
+      if (!MANY || (border != 0 && count_from<V>(x, unordered(border)) <= top_k)) border = 0;
+      break;
+    }
+    border = next;
+    if (key == next) key = 0;
+  }
+  float from = -FLT_MAX;
+  if (border != 0) from = fmaxf(from, unordered(border) - margin * (1.0f + fabsf(unordered(border))));   // never -inf
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mine += x[j] >= from;
+  int n = 0;
+  if constexpr (MANY) n = __reduce_add_sync(kAll, mine);
+  if (MANY && n > kCandidates<true>) {
+    const float closer = closer_border<V>(x, from, unordered(top), top_k);
+    from = fmaxf(from, closer - margin * (1.0f + fabsf(closer)));
+    mine = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) mine += x[j] >= from;
+    n = __reduce_add_sync(kAll, mine);
+    if (n > kCandidates<true>) return n;
+  }
+  // places: lanes before this one with at least 1, 2, ... candidates
+  int at = 0;
+  const unsigned before_me = (1u << lane) - 1;
+  for (int c = 1;; ++c) {
+    const unsigned lanes = __ballot_sync(kAll, mine >= c);
+    if (lanes == 0) break;
+    at += __popc(lanes & before_me);
+    if (!MANY) n += __popc(lanes);
+  }
+  if (!MANY && n > kCandidates<false>) return n;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (x[j] >= from) held[at++] = make_float2(x[j], __int_as_float(expert_of<VEC>(j, lane)));
+  __syncwarp();
+  const float2 last = make_float2(-INFINITY, __int_as_float(0x7fffffff));   // ranks behind all candidates
+  if (lane >= n) held[lane] = last;
+  if (MANY && n > 32 && lane + 32 >= n) held[lane + 32] = last;
+  __syncwarp();
+  const float2 me = held[lane];
+  const int before = before_of(me, held, n);
+  if (MANY && n > 32) {
+    const float2 other = held[lane + 32];
+    const int before_other = before_of(other, held, n);
+    __syncwarp();
+    if (lane + 32 < n) held[before_other] = other;
   }
   __syncwarp();
   if (lane < n) held[before] = me;
@@ -362,7 +422,7 @@ __device__ __forceinline__ int choose(const float (&x)[V], float most, float mar
 // order, or the last choice and the one behind it, are nearer than twice that, 64 bits decide among the candidates
 // (0.3 % of rows for sigmoids of 512 experts).  Experts of equal logit and equal bias have equal scores and need no more
 // digits.  False: too many candidates, nothing is chosen.
-template <class T, int V, int VEC>
+template <bool MANY, class T, int V, int VEC>
 __device__ __forceinline__ bool choose_by_score(const float (&x)[V], const float (&h)[V], float sum, const Rows& a,
                                                 const T* logits, float top, int lane, float2* held, int& expert) {
   const float doubt = a.sigmoid ? 1e-6f : 4e-6f;
@@ -391,8 +451,8 @@ __device__ __forceinline__ bool choose_by_score(const float (&x)[V], const float
   float most = v[0];
 #pragma unroll
   for (int j = 1; j < V; ++j) most = fmaxf(most, v[j]);
-  const int n = choose<V, VEC>(v, most, 2.0f * doubt, a.top_k, lane, held, expert, mine, behind);
-  if (n > 32) return false;
+  const int n = choose<MANY, V, VEC>(v, most, 2.0f * doubt, a.top_k, lane, held, expert, mine, behind);
+  if (n > kCandidates<MANY>) return false;
   float next = __shfl_down_sync(kAll, mine, 1);
   int next_expert = __shfl_down_sync(kAll, expert, 1);
   if (lane >= a.top_k - 1) { next = behind; next_expert = -1; }
@@ -441,7 +501,7 @@ constexpr int kResident = V <= 8 ? 4 : V <= 16 ? 3 : 1;
 // A warp per row, its logits and then its scores in registers: one read of the logits, one exponential a score.  A block
 // walks its chunk of rows with eight warps and the next row on its way; with the loss each warp adds its rows' p in its own
 // part of shared memory (experts slots, no atomics), and counts go through shared whole-number atomics.
-template <class T, int V, int VEC>
+template <class T, int V, int VEC, bool MANY>
 __global__ void __launch_bounds__(kWarps * 32, kResident<V>)
 router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict__ gates, const Records rec) {
   extern __shared__ float4 smem_sums[];                            // (16-byte aligned)
@@ -449,7 +509,7 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
   float* mine = part + (threadIdx.x >> 5) * a.experts;
   int* seen = reinterpret_cast<int*>(part + kWarps * a.experts);   // [experts]
   __shared__ int live_rows[kWarps], live_routes[kWarps];
-  __shared__ float2 held[kWarps][32];
+  __shared__ float2 held[kWarps][kCandidates<MANY>];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool balance = rec.share != nullptr, pick = routes != nullptr;
   const bool whole = balance || a.bias != nullptr || (!a.renormalize && !a.sigmoid);   // scores of all experts
@@ -511,10 +571,11 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
           float logit = 0.0f, behind;
           bool settled;
           if (a.bias != nullptr) {
-            settled = choose_by_score<T, V, VEC>(x, h, sum, a, logits, r.top, lane, held[warp], expert);
+            settled = choose_by_score<MANY, T, V, VEC>(x, h, sum, a, logits, r.top, lane, held[warp], expert);
             if (settled && expert >= 0) logit = as_float(logits[expert]);
           } else {
-            settled = choose<V, VEC>(x, r.lane_top, 0.0f, a.top_k, lane, held[warp], expert, logit, behind) <= 32;
+            settled = choose<MANY, V, VEC>(x, r.lane_top, 0.0f, a.top_k, lane, held[warp], expert, logit, behind) <=
+                      kCandidates<MANY>;
           }
           if (!settled) {
             expert = choose_slowly<T>(logits, a.experts, a.top_k, a.bias, a.sigmoid != 0, r.top, lane);
@@ -902,7 +963,10 @@ Records records_of(const Plan& p, void* workspace, bool counts) {
 template <class T, int V, int VEC>
 void forward_of(const Rows& a, const Plan& p, int* routes, float* gates, const Records& rec, cudaStream_t stream) {
   const int smem = rec.share ? (kWarps + 1) * a.experts * 4 : 0;
-  router_forward_kernel<T, V, VEC><<<p.blocks, kWarps * 32, smem, stream>>>(a, routes, gates, rec);
+  // one lane's worth of experts: every value is a lane's maximum
+  const bool many = V > 1 && routes != nullptr && a.top_k > kFewChoices;
+  auto kernel = many ? router_forward_kernel<T, V, VEC, (V > 1)> : router_forward_kernel<T, V, VEC, false>;
+  kernel<<<p.blocks, kWarps * 32, smem, stream>>>(a, routes, gates, rec);
 }
 template <class T, int V, int VEC>
 void backward_of(const Rows& a, const int* routes, const float* dgates, const float* table, const float* dloss,
