@@ -9,7 +9,7 @@
 // stored, and the accumulation across blocks is plain FP32.
 //
 // "P" is the operand whose rows lie on the TMEM lanes (128 a CTA), "Q" the one whose rows are its columns (BN a tile).
-// P = A, Q = B in general; for few rows of A the roles are swapped (SWAP): the weights' rows fill the lanes and the
+// P = A, Q = B in general; for few rows of A (rides_in_columns) the roles are swapped (SWAP): the weights' rows fill the lanes and the
 // tokens are BN = 16, 32 or 64 columns, so that no lane is idle and the weights stream through once.
 //
 // Warps of a CTA: 0 TMA, 1 MMA and TMEM, 2 and 3 fetch the scales, the others add up the blocks.  A stage's `done`
@@ -759,10 +759,18 @@ Packing packing_of(int m, int n, int kblocks) {
   return k;
 }
 
-// Up to 64 rows of A ride in the columns; beyond that its rows fill the lanes.  CTA pairs take less time a block and
-// wave but start about 2.6 us later (the packing kernel, a pair's set-up), so they pay where they save at least 8 blocks
-// of a wave.  One CTA a tile / pairs, us: 1024 x 4096, K = 512: 8.0 / 8.7, K = 1024: 10.4 / 10.1, K = 4096: 25.4 / 18.2;
-// 2048 x 4096, K = 512: 12.1 / 10.7, K = 4096: 46.6 / 28.8; 2048 x 1024, K = 4096: 14.9 / 17.2.
+// Whether A's rows ride in the columns.  Up to 32 they do; beyond 64 they fill the lanes; between, the narrow tile pays
+// where four CTAs share it, each with 4 to 16 blocks.  64 rows, in the columns / in the lanes, us: 4096 columns of out, K =
+// 1024: 7.0 / 5.9, 2048: 7.8 / 8.4, 4096: 9.3 / 9.9, 16384: 18.1 / 17.3; 16384 columns (one CTA a tile), K = 512: 7.4 / 5.6,
+// 4096: 17.7 / 13.9.
+bool rides_in_columns(int m, int n, int kblocks, int sms) {
+  return m <= 32 || (m <= 64 && (static_cast<long long>(n) + 127) / 128 * 4 <= sms && kblocks >= 16 && kblocks <= 64);
+}
+
+// Beyond 64 rows of A: CTA pairs take less time a block and wave but start about 2.6 us later (the packing kernel, a
+// pair's set-up), so they pay where they save at least 8 blocks of a wave.  One CTA a tile / pairs, us: 1024 x 4096, K =
+// 512: 8.0 / 8.7, K = 1024: 10.4 / 10.1, K = 4096: 25.4 / 18.2; 2048 x 4096, K = 512: 12.1 / 10.7, K = 4096: 46.6 / 28.8;
+// 2048 x 1024, K = 4096: 14.9 / 17.2.
 bool takes_pairs(int m, int n, int kblocks, int sms) {
   if (m <= 64) return false;
   const long long single = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128);
@@ -805,9 +813,11 @@ int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMa
     return WM_ERR_INVALID;
   }
   // Few tiles: 2 or 4 CTAs take a share of the blocks each, while every SM still gets at most one CTA and every CTA
-  // two blocks.  (Clusters of 8 start 2 us later: 1 x 2048 x 4096 took 10.0 us with them, 7.4 us with 4.)
+  // two blocks.  The join costs as much as some blocks: 100 x 1024, K = 1024: 6.0 us alone, 7.5 shared; 2048: 8.3 / 8.1;
+  // 4096: 12.9 / 9.2; one row, K = 512: 4.5 / 4.9, 1024: 5.5 / 4.8.  (Clusters of 8 start 2 us later: 1 x 2048 x 4096 took
+  // 10.0 us with them, 7.4 us with 4.)
   a.split = 1;
-  if (!PAIR)
+  if (!PAIR && a.kblocks >= (SWAP ? 8 : 16))
     while (a.split < 4 && tiles * a.split * 2 <= sms && a.kblocks / (a.split * 2) >= 2) a.split *= 2;
   const int group = PAIR ? 2 : a.split;
   const long long groups = tiles * group <= sms ? tiles : sms / group;
@@ -862,7 +872,7 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   const uint64_t pitch = static_cast<uint64_t>(kblocks) * 128;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const bool swap = m <= 64, pairs = takes_pairs(m, n, kblocks, sms);
+  const bool swap = rides_in_columns(m, n, kblocks, sms), pairs = takes_pairs(m, n, kblocks, sms);
   const int bn = swap ? (m <= 16 ? 16 : m <= 32 ? 32 : 64) : 128;
   const Packing packing = packing_of(m, n, kblocks);
   const bool packed = workspace && pairs;
