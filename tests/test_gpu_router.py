@@ -433,3 +433,24 @@ def test_counts_of_no_tokens(sequences):
     offsets = torch.zeros(sequences + 1, dtype=torch.int32, device="cuda")
     counts = expert_counts(routes, 5, sequences=offsets)
     assert counts.shape == (sequences, 5) and not counts.any()
+
+
+@pytest.mark.parametrize("score, bias", [("softmax", None), ("sigmoid", "zeros"), ("sigmoid", "spread"), ("softmax", "spread")])
+@pytest.mark.parametrize("experts", (33, 64, 300, 512, 1024))
+@pytest.mark.parametrize("top_k", (12, 13, 16, 25, 32))
+def test_many_choices(top_k, experts, score, bias):
+    """More candidates than lanes: plain rows, rows of few distinct values, rows with masked experts, and rows whose
+    values around the border are closer than 32-bit scores tell."""
+    logits = make(40, experts, seed=23)
+    logits[8:16] = (logits[8:16] * 2).round() / 2
+    logits[16] = 0.0
+    logits[17] = logits[17].sign()
+    logits[18, top_k + 1:] = -float("inf")                      # one expert more than choices
+    logits[19, top_k - 2:] = -float("inf")                      # fewer than choices
+    logits[24:32] = 0.25 + torch.arange(experts) * 2.0 ** -24   # neighbours one step apart
+    logits[28:32] = logits[28:32].flip(1)
+    biases = {None: None, "zeros": torch.zeros(experts), "spread": vector(experts, 24, 0.05)}
+    check_route(logits, top_k, bias=biases[bias], score=score)
+    low = torch.full((2, experts), torch.finfo(torch.float32).min)   # apart: it widens the tolerance of the gates
+    low[0, ::3] = 1.0
+    check_route(low, top_k, bias=biases[bias], score=score)

@@ -264,9 +264,9 @@ __device__ __noinline__ int choose_slowly(const T* logits, int experts, int top_
   return expert;
 }
 
-// The n <= 64 candidates in `held` (any order), ranked by their 64-bit scores; lane k gets choice k.  A lane takes one
-// candidate or two, so this costs one exponential in 64 bits or two (and for softmax the row's sum).
-template <class T>
+// The n <= kCandidates candidates in `held` (any order), ranked by their 64-bit scores; lane k gets choice k.  A lane takes
+// one candidate, or two for MANY, so this costs as many exponentials in 64 bits (and for softmax the row's sum).
+template <bool MANY, class T>
 __device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, const float* bias, bool sigmoid,
                                        float top, int lane, float2* held, int n) {
   double sum = 1.0;
@@ -276,23 +276,28 @@ __device__ __noinline__ int rank_in_64(const T* logits, int experts, int top_k, 
     for (int e = lane; e < experts; e += 32) sum += exp(static_cast<double>(as_float(logits[e])) - top);
     sum = warp_sum(sum);
   }
-  int expert[2] = {0x7fffffff, 0x7fffffff}, before[2] = {0, 0};
-  double v[2] = {-INFINITY, -INFINITY};
-  for (int c = 0; c < 2; ++c) {
-    if (lane + 32 * c >= n) break;
+  constexpr int kEach = MANY ? 2 : 1;
+  int expert[kEach], before[kEach];
+  double v[kEach];
+#pragma unroll
+  for (int c = 0; c < kEach; ++c) {
+    expert[c] = 0x7fffffff;
+    before[c] = 0;
+    v[c] = -INFINITY;
+    if (lane + 32 * c >= n) continue;
     expert[c] = __float_as_int(held[lane + 32 * c].y);
     const double x = as_float(logits[expert[c]]);
     v[c] = (sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum) + static_cast<double>(__ldg(bias + expert[c]));
   }
   for (int i = 0; i < n; ++i) {
-    const double w = __shfl_sync(kAll, i < 32 ? v[0] : v[1], i & 31);
-    const int e = __shfl_sync(kAll, i < 32 ? expert[0] : expert[1], i & 31);
+    const double w = __shfl_sync(kAll, i < 32 ? v[0] : v[kEach - 1], i & 31);
+    const int e = __shfl_sync(kAll, i < 32 ? expert[0] : expert[kEach - 1], i & 31);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) before[c] += w > v[c] || (w == v[c] && e < expert[c]);
+    for (int c = 0; c < kEach; ++c) before[c] += w > v[c] || (w == v[c] && e < expert[c]);
   }
   __syncwarp();
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+  for (int c = 0; c < kEach; ++c)
     if (lane + 32 * c < n) held[before[c]].y = __int_as_float(expert[c]);
   __syncwarp();
   const int chosen = lane < min(n, top_k) ? __float_as_int(held[lane].y) : -1;
@@ -337,15 +342,15 @@ __device__ __forceinline__ float closer_border(const float (&x)[V], float border
 // The K largest (value, lowest expert first) of the warp's V x 32 values, `most` the lane's largest; -inf is no
 // candidate.  The (K+1)th largest of the lanes' maxima is at most the (K+1)th largest value, so the values from it up
 // hold the choice and the one behind it; they are few (for unequal values K + 1 and a few lanes' second ones).  They,
-// and with a margin what is at most so much smaller, are gathered in `held` (kCandidates of this warp), and each counts the ones
-// before it.  Lane k gets choice k and its value; `behind` the next value (-inf: none).  Returns the number of
+// and with a margin what is at most so much smaller, are gathered in `held` (kCandidates of this warp), and each counts
+// the ones before it.  Lane k gets choice k and its value; `behind` the next value (-inf: none).  Returns the number of
 // candidates, which stay in `held` in their order; above kCandidates (many equal values) nothing is chosen.
 // MANY: for K above kFewChoices the border of 32 lanes leaves more candidates (24 on average at K = 16, all values at
 // K = 32): room for 64, two a lane, and a border moved up by halving.  65536 x 512 BF16 by logits, with / without: K = 8
 // 80 / 76 us, K = 16 116 / 329, K = 32 202 / 1959; up to 12 the 32 places overflow in less than one row of 10000.
 template <bool MANY, int V, int VEC>
-__device__ __forceinline__ int choose(const float (&x)[V], float most, float margin, int top_k, int lane, float2* held, int& expert,
-                                      float& its, float& behind) {
+__device__ __forceinline__ int choose(const float (&x)[V], float most, float margin, int top_k, int lane, float2* held,
+                                      int& expert, float& its, float& behind) {
   unsigned key = most > -INFINITY ? ordered(most) : 0u, top = 0, border = 0;
   for (int k = 0; k <= top_k; ++k) {   // equal maxima go at once: the border is then lower, which is as good
     const unsigned next = __reduce_max_sync(kAll, key);
@@ -464,7 +469,7 @@ __device__ __forceinline__ bool choose_by_score(const float (&x)[V], const float
                  __ldg(a.bias + expert) != __ldg(a.bias + next_expert);
   }
   if (__any_sync(kAll, doubtful))
-    expert = rank_in_64<T>(logits, a.experts, a.top_k, a.bias, a.sigmoid != 0, top, lane, held, n);
+    expert = rank_in_64<MANY, T>(logits, a.experts, a.top_k, a.bias, a.sigmoid != 0, top, lane, held, n);
   return true;
 }
 
