@@ -85,12 +85,14 @@ __device__ __forceinline__ float power_of_2(float t) {
   return r;
 }
 // Exponentials are powers of 2 of x log2 e.  exp(x - top) is 2^(x log2 e - c) with c the rounded top log2 e: the
-// rounding of c is a factor that all terms of a row share and that their shares do not see, the fused product rounds
-// like the subtraction of the definition.
+// rounding of c, up to half a step of c in the exponent, is a factor that all terms of a row share and that their shares do
+// not see as long as it stays in range.  Up to kFarTop it is at most 2^0.5; from 2^31 on it passes 2^127 and the row's sum
+// would be infinite or 0.  Beyond kFarTop the difference is taken first: it is exact where it counts (logits within a
+// factor of two of top; the others' terms vanish), and its product with log2 e rounds like the fused one.
 constexpr float kLog2E = 1.44269504f;
-constexpr float kHuge = 1e30f;   // beyond it top log2 e may overflow, and differences are 0 or vast
+constexpr float kFarTop = 8388608.0f;   // 2^23: top log2 e is below 2^24, a step of it is at most 1
 __device__ __forceinline__ float exp_below(float x, float top) {
-  return power_of_2(fabsf(top) < kHuge ? fmaf(x, kLog2E, -top * kLog2E) : (x - top) * kLog2E);
+  return power_of_2(fabsf(top) < kFarTop ? fmaf(x, kLog2E, -top * kLog2E) : (x - top) * kLog2E);
 }
 
 struct Rows {
@@ -212,7 +214,7 @@ __device__ __forceinline__ float row_shares(const float (&x)[V], bool sigmoid, f
   float sum = 0.0f;
   if (!sigmoid) {
     const float c = top * kLog2E;
-    if (fabsf(top) < kHuge) {
+    if (fabsf(top) < kFarTop) {
 #pragma unroll
       for (int j = 0; j < V; ++j) { h[j] = power_of_2(fmaf(x[j], kLog2E, -c)); sum += h[j]; }
     } else {
