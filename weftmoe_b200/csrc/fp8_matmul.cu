@@ -369,8 +369,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
     tma_prefetch_desc(&tmap_q);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, S::kColumns);
-    tmem_relinquish();
+    tmem_alloc<PAIR ? 2 : 1>(tmem_holder, S::kColumns);   // PAIR: warp 1 of both CTAs, as all of the kernel's group
+    tmem_relinquish<PAIR ? 2 : 1>();
   }
   tc_fence_before();
   __syncthreads();
@@ -694,7 +694,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
   if constexpr (PAIR) cluster_sync_all();  // the peer's shared memory and barriers stay valid until both are done
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, S::kColumns);
+    tmem_dealloc<PAIR ? 2 : 1>(tmem_base, S::kColumns);
   }
   if (!PAIR && a.split > 1) cluster_wait();   // this CTA's sums stay until the others have read them
 }

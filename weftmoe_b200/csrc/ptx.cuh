@@ -172,18 +172,31 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
 }
 
 // ---------------------------------------------------------------- tcgen05 / TMEM
+// GROUP: the CTA group that all tcgen05 instructions of the kernel name.  2: one warp of each CTA of the pair executes
+// these together, and both get the same columns.
+template <int GROUP = 1>
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_holder, uint32_t columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(smem_holder)),
-               "r"(columns)
-               : "memory");
+  static_assert(GROUP == 1 || GROUP == 2, "CTA group");
+  if constexpr (GROUP == 2)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_holder)),
+                 "r"(columns)
+                 : "memory");
+  else
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_holder)),
+                 "r"(columns)
+                 : "memory");
 }
+template <int GROUP = 1>
 __device__ __forceinline__ void tmem_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if constexpr (GROUP == 2) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  else asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
+template <int GROUP = 1>
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(columns)
-               : "memory");
+  if constexpr (GROUP == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(columns) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
