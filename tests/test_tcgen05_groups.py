@@ -24,7 +24,7 @@ def test_tmem_helpers_come_in_both_groups():
             assert f"tcgen05.{instruction}.cta_group::{group}.sync.aligned" in text, (instruction, group)
 
 
-@pytest.mark.parametrize("name, group", [("fp8_matmul.cu", "<PAIR ? 2 : 1>")])
+@pytest.mark.parametrize("name, group", [("fp8_matmul.cu", "<PAIR ? 2 : 1>"), ("gemm2.cuh", "<2>")])
 def test_pair_kernels_take_their_tmem_as_a_pair(name, group):
     calls = tmem_calls(name)
     assert sorted(c for c, _ in calls) == ["alloc", "dealloc", "relinquish"]

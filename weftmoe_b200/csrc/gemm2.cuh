@@ -124,10 +124,10 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__
     tma_prefetch_desc(&tmap_b);
   }
   if (warp == 1) {
-    // Each CTA takes all of its own TMEM, so both allocations start at column 0 and the pair
-    // MMA can address the two accumulators with one address.
-    tmem_alloc(tmem_holder, kTmemCols == 512 ? 512 : 256);
-    tmem_relinquish();
+    // The two CTAs allocate together and get the same columns, so the pair
+    // MMA addresses the two accumulators with one address.
+    tmem_alloc<2>(tmem_holder, kTmemCols == 512 ? 512 : 256);
+    tmem_relinquish<2>();
   }
   tc_fence_before();
   __syncthreads();
@@ -258,7 +258,7 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__
   cluster_sync_all();  // the peer's shared memory and barriers stay valid until both are done
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, kTmemCols == 512 ? 512 : 256);
+    tmem_dealloc<2>(tmem_base, kTmemCols == 512 ? 512 : 256);
   }
 }
 
