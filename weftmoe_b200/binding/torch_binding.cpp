@@ -24,12 +24,13 @@ void check(int code) {
   TORCH_CHECK(false, message);
 }
 
-// The current stream of the tensors' device, made current; storage of tensors from another stream is kept for it.
+// The current stream of the tensors' device, made current; storage of tensors from another stream that the call uses
+// (reads or, where the caller gives a result, writes) is kept for it.
 struct Launch {
   c10::cuda::CUDAGuard guard;
   c10::cuda::CUDAStream stream;
   explicit Launch(const Tensor& like) : guard(like.device()), stream(c10::cuda::getCurrentCUDAStream()) {}
-  void reads(const Tensor& t) {
+  void uses(const Tensor& t) {
     if (t.defined() && t.numel() > 0) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), stream);
   }
   operator void*() const { return static_cast<void*>(stream.stream()); }
@@ -101,7 +102,7 @@ variable_list route_forward(const Tensor& rows, const Choice& c, const Tensor& b
   const wm_router r = describe(rows, c, bias, padding, sequences);
   Tensor routes = at::empty({rows.size(0), c.top_k}, rows.options().dtype(at::kInt));
   Tensor gates = at::empty({rows.size(0), c.top_k}, rows.options().dtype(at::kFloat));
-  for (const Tensor& t : {rows, bias, padding, sequences}) launch.reads(t);
+  for (const Tensor& t : {rows, bias, padding, sequences}) launch.uses(t);
   if (!balance) {
     check(wm_router_forward(&r, data<int32_t>(routes), data<float>(gates), nullptr, nullptr, nullptr, nullptr, 0, launch));
     return {routes, gates};
@@ -120,7 +121,7 @@ std::pair<Tensor, Tensor> balance_forward(const Tensor& rows, const Tensor& coun
   c.score = score;
   const wm_router r = describe(rows, c, Tensor(), padding, sequences);
   Loss l(rows, r);
-  for (const Tensor& t : {rows, counts, padding, sequences}) launch.reads(t);
+  for (const Tensor& t : {rows, counts, padding, sequences}) launch.uses(t);
   check(wm_balance_forward(&r, data<int32_t>(counts), data<float>(l.loss), data<float>(l.table), l.workspace.data_ptr(),
                            l.workspace.numel(), launch));
   return {l.loss, l.table};
@@ -136,7 +137,7 @@ Tensor router_backward(const Tensor& rows, const Choice& c, const Tensor& paddin
   if (loss_part) dloss = dloss.to(at::kFloat).contiguous();
   const wm_router r = describe(rows, c, Tensor(), padding, sequences);
   Tensor dlogits = at::empty(rows.sizes(), rows.options());
-  for (const Tensor& t : {rows, padding, sequences, routes, dgates, table, dloss}) launch.reads(t);
+  for (const Tensor& t : {rows, padding, sequences, routes, dgates, table, dloss}) launch.uses(t);
   check(wm_router_backward(&r, gates_part ? data<int32_t>(routes) : nullptr, data<float>(dgates),
                            loss_part ? data<float>(table) : nullptr, data<float>(dloss), dlogits.data_ptr(), launch));
   return dlogits;
@@ -225,8 +226,8 @@ Tensor expert_counts(const Tensor& routes, int64_t experts, const optional<Tenso
   Launch launch(routes);
   const Tensor seq = or_none(sequences);
   Tensor counts = empty_counts(routes, experts, seq);
-  launch.reads(routes);
-  launch.reads(seq);
+  launch.uses(routes);
+  launch.uses(seq);
   check(wm_expert_counts(data<int32_t>(routes), static_cast<int32_t>(routes.size(0)), static_cast<int32_t>(routes.size(1)),
                          static_cast<int32_t>(experts), data<int32_t>(seq),
                          seq.defined() ? static_cast<int32_t>(seq.numel() - 1) : 0, data<int32_t>(counts), launch));
@@ -251,7 +252,7 @@ void matmul_into(Launch& launch, const Tensor& a, const Tensor& as, int64_t a_bl
   check(wm_fp8_matmul_workspace(static_cast<int32_t>(m), static_cast<int32_t>(n), static_cast<int32_t>(k), &bytes));
   Tensor workspace;
   if (bytes) workspace = at::empty({bytes}, as.options().dtype(at::kByte));
-  for (const Tensor& t : {a, as, b, bs}) launch.reads(t);
+  for (const Tensor& t : {a, as, b, bs}) launch.uses(t);
   check(wm_fp8_matmul(a.data_ptr(), data<float>(as), b.data_ptr(), data<float>(bs), out.data_ptr(), ld,
                       static_cast<int32_t>(m), static_cast<int32_t>(n), static_cast<int32_t>(k),
                       static_cast<int32_t>(a_block_rows), static_cast<int32_t>(b_block_rows), is_f32(out), accumulate,
@@ -263,6 +264,7 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& as, int64_t a_block_rows, const
                   bool accumulate) {
   Launch launch(as);
   Tensor out = given.has_value() ? *given : at::empty({m, n}, as.options().dtype(out_is_f32 ? at::kFloat : at::kBFloat16));
+  if (given.has_value()) launch.uses(out);
   matmul_into(launch, a, as, a_block_rows, b, bs, b_block_rows, out, m > 1 ? out.stride(0) : std::max<int64_t>(n, 1), m, n,
               k, accumulate);
   if (given.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
@@ -273,14 +275,14 @@ void quantise_both(Launch& launch, const Tensor& x, Quantised& rows, Quantised& 
   const int64_t m = x.size(0), k = x.size(1);
   rows = Quantised(x, m, k);
   columns = Quantised(x, k, m);
-  launch.reads(x);
+  launch.uses(x);
   check(wm_fp8_quantize_both(x.data_ptr(), is_f32(x), 1, static_cast<int32_t>(m), static_cast<int32_t>(k),
                              rows.values.data_ptr(), data<float>(rows.scales), columns.values.data_ptr(),
                              data<float>(columns.scales), launch));
 }
 Quantised quantise(Launch& launch, const Tensor& x, bool transpose) {
   Quantised q(x, x.size(transpose ? 1 : 0), x.size(transpose ? 0 : 1));
-  launch.reads(x);
+  launch.uses(x);
   check(wm_fp8_quantize(x.data_ptr(), is_f32(x), 1, static_cast<int32_t>(x.size(0)), static_cast<int32_t>(x.size(1)), 1,
                         transpose, q.values.data_ptr(), data<float>(q.scales), launch));
   return q;
@@ -294,7 +296,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& wq, const Tensor& ws, int64
   check(wm_fp8_linear_workspace(rows, static_cast<int32_t>(n), k, &bytes));
   Tensor y = at::empty({x.size(0), n}, x.options());
   Tensor workspace = at::empty({bytes}, x.options().dtype(at::kByte));
-  for (const Tensor& t : {x, wq, ws}) launch.reads(t);
+  for (const Tensor& t : {x, wq, ws}) launch.uses(t);
   check(wm_fp8_linear(x.data_ptr(), is_f32(x), rows, k, wq.data_ptr(), data<float>(ws), static_cast<int32_t>(n),
                       y.data_ptr(), workspace.data_ptr(), bytes, launch));
   return y;
