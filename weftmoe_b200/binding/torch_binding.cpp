@@ -40,6 +40,12 @@ void refuse_second_derivative(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated again");
 }
 
+// Inputs of forward-mode differentiation need not require a gradient, so they would pass as constants and the
+// results would lack their tangents.
+void refuse_tangent(const char* what, const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, " has no derivative in forward mode");
+}
+
 template <class T>
 T* data(const Tensor& t) {
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
@@ -208,6 +214,7 @@ bool wants_gradient(const Tensor& t) { return at::GradMode::is_enabled() && t.re
 variable_list route(const Tensor& logits, int64_t top_k, int64_t score, bool renormalize, double scale,
                     const optional<Tensor>& bias, const optional<Tensor>& padding, const optional<Tensor>& sequences,
                     bool balance) {
+  refuse_tangent("The router", logits);
   const Choice c{top_k, score, renormalize, scale};
   if (wants_gradient(logits))
     return Route::apply(logits, c, bias, padding, sequences, balance);
@@ -218,6 +225,7 @@ variable_list route(const Tensor& logits, int64_t top_k, int64_t score, bool ren
 
 Tensor balance(const Tensor& logits, const Tensor& counts, int64_t score, const optional<Tensor>& padding,
                const optional<Tensor>& sequences) {
+  refuse_tangent("balance_loss", logits);
   if (wants_gradient(logits)) return Balance::apply(logits, counts, score, padding, sequences);
   return balance_forward(rows_of(logits), counts, score, or_none(padding), or_none(sequences)).first;
 }
@@ -351,6 +359,8 @@ struct Linear : torch::autograd::Function<Linear> {
 
 Tensor fp8_linear(const Tensor& x, const Tensor& weight, const Tensor& wq, const Tensor& ws, const optional<Tensor>& wtq,
                   const optional<Tensor>& wts) {
+  refuse_tangent("fp8_linear", x);
+  refuse_tangent("fp8_linear", weight);
   const bool to_weight = wants_gradient(weight);
   if (wants_gradient(x) || to_weight) return Linear::apply(x, weight, wq, ws, wtq, wts, to_weight);
   return linear_forward(x, wq, ws, weight.size(0));

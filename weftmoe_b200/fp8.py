@@ -425,8 +425,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, prepared: PreparedFP8Linea
 
     x (BF16 or FP32; y has its type) is quantised 1 x 128, the weight comes quantised 128 x 128 from
     `prepare_fp8_linear(weight)`.  Backward: dx from dy in 1 x 128 blocks and the same weight bytes; dW (of the
-    weight's type) from dy and x in 1 x 128 blocks along the tokens.  Capture a backward pass together with its
-    forward pass."""
+    weight's type) from dy and x in 1 x 128 blocks along the tokens; forward mode and second derivatives are refused.
+    Capture a backward pass together with its forward pass."""
     if not isinstance(prepared, PreparedFP8Linear):
         raise TypeError("prepared must be PreparedFP8Linear")
     if not isinstance(x, torch.Tensor) or x.dtype not in _SOURCE_DTYPES or x.ndim < 1:

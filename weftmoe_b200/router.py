@@ -9,7 +9,8 @@ The reference leaves the router to its host framework (weftmoe/megatron.py:164-1
 the definitions are in include/weftmoe_b200.h beside `wm_router`.  All arithmetic runs in libweftmoe_b200.so; this
 file checks arguments, binding/torch_binding.cpp allocates results and joins the calls to autograd.  Every call enqueues on the current
 stream of the logits' device, synchronises nothing and may be captured in a CUDA graph; capture a backward pass
-together with its forward pass (autograd runs a backward pass on the stream of its forward pass).
+together with its forward pass (autograd runs a backward pass on the stream of its forward pass).  First derivatives in
+reverse mode: forward mode and second derivatives are refused.
 """
 from __future__ import annotations
 
