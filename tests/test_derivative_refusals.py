@@ -4,8 +4,8 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from weftmoe_b200 import _lib
-from weftmoe_b200.fp8 import fp8_linear, prepare_fp8_linear
+from weftmoe_b200 import _lib, fp8
+from weftmoe_b200.fp8 import fp8_linear, fp8_matmul, prepare_fp8_linear, quantize_fp8
 from weftmoe_b200.router import balance_loss, expert_counts, route_and_balance, route_tokens
 
 
@@ -58,3 +58,35 @@ def test_second_derivatives_are_refused():
                         (route_and_balance(x, 2)[3], x), (fp8_linear(y, weight, prepare_fp8_linear(weight)).sum(), y)):
         with pytest.raises(RuntimeError, match="cannot be differentiated again"):
             torch.autograd.grad(value, leaf, create_graph=True)
+
+
+def outs_with_history(device):
+    leaf = torch.zeros(8, 16, device=device, requires_grad=True)
+    return leaf, leaf * 2, leaf[:, :], (torch.zeros(8, 32, device=device, requires_grad=True) + 1)[:, 8:24]
+
+
+@pytest.mark.parametrize("accumulate", (False, True))
+def test_an_out_with_a_gradient_is_refused(accumulate):
+    a, b = (fp8._allocate((rows, 256), 1, torch.empty(0)) for rows in (8, 16))
+    for out in outs_with_history("cpu"):
+        before = out._version
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            fp8_matmul(a, b, dtype=torch.float32, out=out, accumulate=accumulate)
+        assert out._version == before
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+        fp8_matmul(a, b, dtype=torch.float32, out=dual(8, 16))
+
+
+@pytest.mark.gpu
+def test_an_out_without_a_gradient_is_taken():
+    a, b = (quantize_fp8(torch.randn(rows, 256, device="cuda", dtype=torch.bfloat16)) for rows in (8, 16))
+    want = fp8_matmul(a, b, dtype=torch.float32)
+    for out in outs_with_history("cuda"):
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            fp8_matmul(a, b, dtype=torch.float32, out=out)
+        with torch.no_grad():                                     # the caller's own part, as for torch's calls
+            assert torch.equal(fp8_matmul(a, b, dtype=torch.float32, out=out), want)
+    leaf = torch.zeros(8, 16, device="cuda", requires_grad=True)
+    leaf.grad = torch.ones(8, 16, device="cuda")
+    fp8_matmul(a, b, dtype=torch.float32, out=leaf.grad, accumulate=True)
+    assert torch.equal(leaf.grad, want + 1)

@@ -270,6 +270,8 @@ void matmul_into(Launch& launch, const Tensor& a, const Tensor& as, int64_t a_bl
 Tensor fp8_matmul(const Tensor& a, const Tensor& as, int64_t a_block_rows, const Tensor& b, const Tensor& bs,
                   int64_t b_block_rows, int64_t m, int64_t n, int64_t k, bool out_is_f32, const optional<Tensor>& given,
                   bool accumulate) {
+  for (const Tensor& t : {as, bs, or_none(given)})
+    if (t.defined()) refuse_tangent("fp8_matmul", t);
   Launch launch(as);
   Tensor out = given.has_value() ? *given : at::empty({m, n}, as.options().dtype(out_is_f32 ? at::kFloat : at::kBFloat16));
   if (given.has_value()) launch.uses(out);

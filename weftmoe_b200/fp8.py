@@ -195,7 +195,9 @@ def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.T
     """A @ B^T of A [M, K] and B [N, K], blocks of 1 or 128 rows on either side, any scales.
 
     Enqueues on the current stream and returns; may be captured.  `out` (BF16 or FP32 like `dtype`) may be a
-    slice of a wider tensor: unit column stride, rows at least N apart; writing it counts as a change in place.  `accumulate` adds into an FP32 `out`."""
+    slice of a wider tensor: unit column stride, rows at least N apart; writing it counts as a change in place.
+    `accumulate` adds into an FP32 `out`.  Not differentiable; an `out` that requires a gradient is refused while gradients
+    are enabled (a `.grad` does not require one)."""
     if not isinstance(a, FP8Tensor) or not isinstance(b, FP8Tensor):
         raise TypeError("fp8_matmul takes FP8Tensor operands")
     if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[1] or a.data.device != b.data.device:
@@ -210,6 +212,8 @@ def fp8_matmul(a: FP8Tensor, b: FP8Tensor, *, dtype=torch.bfloat16, out: torch.T
                 and out.device == a.data.device and (n <= 1 or out.stride(1) == 1) and (m <= 1 or out.stride(0) >= n))
         if not fits:
             raise ValueError("FP8 output shape, dtype, device or layout mismatch")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("fp8_matmul is not differentiable: it cannot write an `out` that requires a gradient")
     product = _lib.binding().fp8_matmul(a.data, a.scales, a.block_rows, b.data, b.scales, b.block_rows, m, n, k,
                                         dtype == torch.float32, out, accumulate)
     return product if out is None else out
