@@ -376,6 +376,10 @@ WM_API int wm_debug_grouped_gemm(int kind, const void* a, const void* b, void* o
  * tile heuristic lives in weftmoe/blackwell_cutlass.py:80-88. */
 WM_API void wm_debug_force_gemm_pairs(int mode);
 
+/* Diagnostic: have wm_fp8_matmul take its CTA-pair kernels as built with at most `most` registers a thread (<= 0: as they
+ * are).  Below what their warps share out among them, every product goes to the one-CTA kernels. */
+WM_API void wm_debug_matmul_pair_registers(int most);
+
 /* Diagnostics of the bounded cross-rank waits (reference: the transport deadline,
  * ActivationTransportRunOptions.deadline_after -> NotifyErrorCode::TransportTimeout,
  * include/weftmoe/cuda/activation_transport.hpp:169-175, src/cuda/activation_transport/execution.cuh:1243-1250).

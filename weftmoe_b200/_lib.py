@@ -96,6 +96,7 @@ SIGNATURES = {
     "wm_router_backward": (c_int, [POINTER(WmRouter)] + [c_void_p] * 6),
     "wm_expert_counts": (c_int, [c_void_p] + [c_int32] * 3 + [c_void_p, c_int32, c_void_p, c_void_p]),
     "wm_debug_force_gemm_pairs": (None, [c_int]),
+    "wm_debug_matmul_pair_registers": (None, [c_int]),
     "wm_debug_set_wait_budget": (c_int, [ctypes.c_longlong]),
     "wm_debug_wait_flag": (c_int, [c_void_p, c_void_p, c_int32, c_void_p]),
     "wm_debug_grouped_gemm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

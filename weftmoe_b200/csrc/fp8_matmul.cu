@@ -32,6 +32,11 @@
 // the power limit makes it 116 us.  Long K on few tiles (4096 x 2048, K = 8190: 57 us, 60 % busy): 128 tiles on 74 pairs,
 // a second wave that is three quarters full.  General scales on pairs (147 and 154 us for these two): the adding warps, 128
 // accumulators a thread read, scaled and added for every block.
+#include <limits.h>
+
+#include <algorithm>
+#include <atomic>
+
 #include "../../include/weftmoe_b200.h"
 #include "gemm.cuh"
 #include "kernels.h"
@@ -210,7 +215,7 @@ struct Matmul {
   static constexpr uint32_t kTmemScales = BN;
   static_assert(!PAIR || kStages * kPackedBytes <= kScaleBytes, "packed scales fit where the table is");
   // PAIR: the four service warps give registers to the eight adding warps: 128 x 56 + 256 x 224 = 384 x 168, what
-  // the block is launched with (checked before the first launch).
+  // the block is launched with (pair_kernels_fit looks before a launch is planned).
   static constexpr int kRegisters = 168, kLow = 56, kHigh = 224;
   static_assert(!PAIR || 128 * kLow + 256 * kHigh <= kThreads * kRegisters, "registers of the block");
 };
@@ -771,12 +776,30 @@ bool rides_in_columns(int m, int n, int kblocks, int sms) {
 // pair's set-up), so they pay where they save at least 8 blocks of a wave.  One CTA a tile / pairs, us: 1024 x 4096, K =
 // 512: 8.0 / 8.7, K = 1024: 10.4 / 10.1, K = 4096: 25.4 / 18.2; 2048 x 4096, K = 512: 12.1 / 10.7, K = 4096: 46.6 / 28.8;
 // 2048 x 1024, K = 4096: 14.9 / 17.2.
-bool takes_pairs(int m, int n, int kblocks, int sms) {
+bool pays_for_pairs(int m, int n, int kblocks, int sms) {
   if (m <= 64) return false;
   const long long single = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128);
   const long long paired = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256);
   const long long waves = (single + sms - 1) / sms - (paired + sms / 2 - 1) / (sms / 2);
   return waves * kblocks >= 8;
+}
+
+// Whether both pair kernels were built with the registers that their warps share out: the launch bounds are only a
+// limit from above, and warps that asked for more than the block has would wait for good.
+std::atomic<int> g_most_registers{INT_MAX};   // wm_debug_matmul_pair_registers
+int pair_kernels_fit(bool* fit) {
+  using S = Matmul<256, 8, false, true, true>;
+  static std::atomic<int> built{0};   // the lower of the two; 0 = not asked yet
+  int registers = built.load(std::memory_order_relaxed);
+  if (registers == 0) {
+    cudaFuncAttributes by_column{}, by_block{};
+    WM_CUDA(cudaFuncGetAttributes(&by_column, fp8_matmul_kernel<256, 8, false, true, true>));
+    WM_CUDA(cudaFuncGetAttributes(&by_block, fp8_matmul_kernel<256, 8, false, false, true>));
+    registers = std::min(by_column.numRegs, by_block.numRegs);
+    built.store(registers, std::memory_order_relaxed);
+  }
+  *fit = std::min(registers, g_most_registers.load(std::memory_order_relaxed)) >= S::kRegisters;
+  return WM_OK;
 }
 
 int sm_count(int* sms) {
@@ -786,6 +809,11 @@ int sm_count(int* sms) {
   return WM_OK;
 }
 
+int takes_pairs(int m, int n, int kblocks, int sms, bool* pairs) {
+  *pairs = pays_for_pairs(m, n, kblocks, sms);
+  return *pairs ? pair_kernels_fit(pairs) : WM_OK;
+}
+
 template <int BN, int EPI, bool SWAP, bool Q_COLS, bool PAIR>
 int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tout, const CUtensorMap& tsp,
                   const CUtensorMap& tsq, MatmulArgs a, int sms, cudaStream_t stream) {
@@ -793,18 +821,6 @@ int launch_matmul(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMa
   auto kernel = fp8_matmul_kernel<BN, EPI, SWAP, Q_COLS, PAIR>;
   static PerDeviceOnce configured;  // one table per template instantiation
   if (int rc = opt_in_dynamic_smem(kernel, S::kTotal, configured)) return rc;
-  if constexpr (PAIR) {
-    static int registers = 0;   // what the kernel was built with
-    if (registers == 0) {
-      cudaFuncAttributes attributes{};
-      WM_CUDA(cudaFuncGetAttributes(&attributes, kernel));
-      registers = attributes.numRegs;
-    }
-    if (registers != S::kRegisters) {
-      set_error("wm_fp8_matmul: the kernel was built with %d registers, its warps share out %d", registers, S::kRegisters);
-      return WM_ERR_STATE;
-    }
-  }
   a.p_tiles = (a.p_rows + S::kRowsP - 1) / S::kRowsP;
   a.q_tiles = (a.q_rows + BN - 1) / BN;
   const long long tiles = static_cast<long long>(a.p_tiles) * a.q_tiles;
@@ -872,7 +888,9 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   const uint64_t pitch = static_cast<uint64_t>(kblocks) * 128;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const bool swap = rides_in_columns(m, n, kblocks, sms), pairs = takes_pairs(m, n, kblocks, sms);
+  const bool swap = rides_in_columns(m, n, kblocks, sms);
+  bool pairs = false;
+  if (int rc = takes_pairs(m, n, kblocks, sms, &pairs)) return rc;
   const int bn = swap ? (m <= 16 ? 16 : m <= 32 ? 32 : 64) : 128;
   const Packing packing = packing_of(m, n, kblocks);
   const bool packed = workspace && pairs;
@@ -974,8 +992,14 @@ extern "C" int wm_fp8_matmul_workspace(int32_t m, int32_t n, int32_t k, int64_t*
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int kblocks = static_cast<int>((static_cast<long long>(k) + 127) / 128);
-  *bytes = takes_pairs(m, n, kblocks, sms) ? packing_of(m, n, kblocks).bytes : 0;
+  bool pairs = false;
+  if (int rc = takes_pairs(m, n, kblocks, sms, &pairs)) return rc;
+  *bytes = pairs ? packing_of(m, n, kblocks).bytes : 0;
   return WM_OK;
+}
+
+extern "C" void wm_debug_matmul_pair_registers(int most) {
+  g_most_registers.store(most > 0 ? most : INT_MAX, std::memory_order_relaxed);
 }
 
 extern "C" int wm_fp8_matmul_status(int32_t* code, void* stream_) {
