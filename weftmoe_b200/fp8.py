@@ -396,11 +396,13 @@ class PreparedFP8Linear:
 
     def wait(self):
         """Order the current stream after the preparation kernels, until they are known to be done."""
-        if self._ready is not None and not torch.cuda.is_current_stream_capturing():
-            if self._ready.query():
-                self._ready = None
-            else:
-                torch.cuda.current_stream(self.weight.data.device).wait_event(self._ready)
+        ready = self._ready                     # another thread may find it done, and drop it, meanwhile
+        if ready is None or torch.cuda.is_current_stream_capturing():
+            return
+        if ready.query():
+            self._ready = None
+        else:
+            torch.cuda.current_stream(self.weight.data.device).wait_event(ready)
 
 
 @torch.inference_mode(False)
