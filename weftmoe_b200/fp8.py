@@ -372,15 +372,19 @@ def prepare_fp8_weights(w1, w2, *, training: bool = True, version: int = 0) -> P
 
 class PreparedFP8Linear:
     """One version of a projection's weight [out, in] in 128 x 128 blocks, and its transpose (the same bytes and
-    scales) for the gradient of the input when prepared for training.  Prepare a new one after each optimizer step."""
+    scales) for the gradient of the input when prepared for training.  Prepare a new one after each optimizer step; a
+    preparation that is captured in a CUDA graph is repeated by every replay."""
 
     __slots__ = ("weight", "weight_t", "_ready", "_stamps", "_origin", "__weakref__")
 
     def __init__(self, weight, weight_t, origin):
         self.weight, self.weight_t, self._origin = weight, weight_t, origin
         with torch.cuda.device(weight.data.device):
-            self._ready = torch.cuda.Event()
-            self._ready.record()                # preparation kernels were enqueued on this stream
+            if torch.cuda.is_current_stream_capturing():
+                self._ready = None              # the graph's replays prepare it; who comes behind them, the caller orders
+            else:
+                self._ready = torch.cuda.Event()
+                self._ready.record()            # preparation kernels were enqueued on this stream
         self._stamps = self._versions()
 
     def _versions(self):
