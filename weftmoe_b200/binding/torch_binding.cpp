@@ -251,6 +251,12 @@ struct Quantised {
         scales(at::empty({rows, (k + 127) / 128}, like.options().dtype(at::kFloat))) {}
 };
 
+// The C ABI takes sizes in 32 bits.
+void check_sizes(std::initializer_list<int64_t> sizes) {
+  for (const int64_t n : sizes)
+    TORCH_CHECK_VALUE(n >= 0 && n < (int64_t{1} << 31), "FP8 matrices must have fewer than 2^31 rows and columns");
+}
+
 int is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 
 // out[m][n] (+)= A[m][k] B[n][k]^T on the current device and stream
@@ -272,6 +278,7 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& as, int64_t a_block_rows, const
                   bool accumulate) {
   for (const Tensor& t : {as, bs, or_none(given)})
     if (t.defined()) refuse_tangent("fp8_matmul", t);
+  check_sizes({m, n, k});
   Launch launch(as);
   Tensor out = given.has_value() ? *given : at::empty({m, n}, as.options().dtype(out_is_f32 ? at::kFloat : at::kBFloat16));
   if (given.has_value()) launch.uses(out);
@@ -363,6 +370,7 @@ Tensor fp8_linear(const Tensor& x, const Tensor& weight, const Tensor& wq, const
                   const optional<Tensor>& wts) {
   refuse_tangent("fp8_linear", x);
   refuse_tangent("fp8_linear", weight);
+  check_sizes({x.size(0), x.size(1), weight.size(0)});
   const bool to_weight = wants_gradient(weight);
   if (wants_gradient(x) || to_weight) return Linear::apply(x, weight, wq, ws, wtq, wts, to_weight);
   return linear_forward(x, wq, ws, weight.size(0));

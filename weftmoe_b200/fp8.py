@@ -98,8 +98,15 @@ def _swap_last_two(shape):
     return (*shape[:-2], shape[-1], shape[-2])
 
 
+def _check_sizes(shape):
+    """The C ABI takes sizes in 32 bits."""
+    if any(n >= 2 ** 31 for n in shape):
+        raise ValueError("FP8 matrices must have fewer than 2^31 rows and columns")
+
+
 def _source_args(tensor):
     """(pointer, is_fp32, batches, rows, cols) of a BF16/FP32 source for the C ABI."""
+    _check_sizes(tensor.shape)
     batches = tensor.shape[0] if tensor.ndim == 3 else 1
     return _lib.ptr(tensor), int(tensor.dtype == torch.float32), batches, tensor.shape[-2], tensor.shape[-1]
 
@@ -416,6 +423,7 @@ def prepare_fp8_linear(weight, *, training: bool = True) -> PreparedFP8Linear:
     if isinstance(weight, FP8Tensor):
         if len(weight.shape) != 2:
             raise ValueError("Expected a weight [out, in]")
+        _check_sizes(weight.shape)
         straight = _import_quantised(weight)
         with torch.cuda.device(straight.data.device):
             flipped = transpose_fp8_weight(straight) if training else None
