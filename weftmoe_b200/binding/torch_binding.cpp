@@ -3,6 +3,7 @@
 // as Python autograd functions the calls took 98 (router), 130 (balance loss) and 160 us (router step) on the host,
 // several times what the GPU needs.  Arguments are checked by router.py and fp8.py before they get here.
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -211,10 +212,26 @@ struct Balance : torch::autograd::Function<Balance> {
 
 bool wants_gradient(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// In a capture: a leaf whose gradient an eager graph, still alive, accumulates on the legacy default stream.  That stream
+// cannot join a capture, and the captured backward pass, which would have to wait for it, fails inside autograd and can
+// take the process along; so the forward pass is refused.
+void refuse_eager_leaf(const char* what, const Tensor& t) {
+  if (!t.is_cuda() || !wants_gradient(t) || !t.is_leaf()) return;
+  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!held) return;
+  const optional<c10::Stream> stream = held->stream();
+  if (!stream.has_value() || *stream != c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap()) return;
+  const c10::cuda::CUDAGuard guard(t.device());
+  TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None, what,
+              ": an eager graph of this leaf on the default stream is alive; drop its results before a capture, or make "
+              "them on a side stream");
+}
+
 variable_list route(const Tensor& logits, int64_t top_k, int64_t score, bool renormalize, double scale,
                     const optional<Tensor>& bias, const optional<Tensor>& padding, const optional<Tensor>& sequences,
                     bool balance) {
   refuse_tangent("The router", logits);
+  refuse_eager_leaf("The router", logits);
   const Choice c{top_k, score, renormalize, scale};
   if (wants_gradient(logits))
     return Route::apply(logits, c, bias, padding, sequences, balance);
@@ -226,6 +243,7 @@ variable_list route(const Tensor& logits, int64_t top_k, int64_t score, bool ren
 Tensor balance(const Tensor& logits, const Tensor& counts, int64_t score, const optional<Tensor>& padding,
                const optional<Tensor>& sequences) {
   refuse_tangent("balance_loss", logits);
+  refuse_eager_leaf("balance_loss", logits);
   if (wants_gradient(logits)) return Balance::apply(logits, counts, score, padding, sequences);
   return balance_forward(rows_of(logits), counts, score, or_none(padding), or_none(sequences)).first;
 }
@@ -371,6 +389,8 @@ Tensor fp8_linear(const Tensor& x, const Tensor& weight, const Tensor& wq, const
   refuse_tangent("fp8_linear", x);
   refuse_tangent("fp8_linear", weight);
   check_sizes({x.size(0), x.size(1), weight.size(0)});
+  refuse_eager_leaf("fp8_linear", x);
+  refuse_eager_leaf("fp8_linear", weight);
   const bool to_weight = wants_gradient(weight);
   if (wants_gradient(x) || to_weight) return Linear::apply(x, weight, wq, ws, wtq, wts, to_weight);
   return linear_forward(x, wq, ws, weight.size(0));
