@@ -49,3 +49,14 @@ def test_projection_without_pairs(too_few_registers):
     x = torch.randint(-4, 5, (M, K), device="cuda").bfloat16()
     y = fp8_linear(x, weight, prepare_fp8_linear(weight, training=False))
     assert torch.equal(y, (x.double() @ weight.double().t()).bfloat16())
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("a_rows, b_rows", [(128, 1), (128, 128)])
+@pytest.mark.parametrize("m, n, k", [(M, N, K), (1408, 1665, 2048), (4100, 4200, 640)])
+def test_packed_scales_of_128_rows_on_the_left(m, n, k, a_rows, b_rows, dtype):
+    """Power-of-two scales of 128 rows of A on the tensor cores, also where the last 128 or 256 rows are not full."""
+    assert workspace(m, n, k) > 0
+    a, b = operand(m, k, a_rows, 62), operand(n, k, b_rows, 63)
+    assert torch.equal(fp8_matmul(a, b, dtype=dtype), (wide(a) @ wide(b).t()).float().to(dtype))
+    poll_fp8_matmul()
