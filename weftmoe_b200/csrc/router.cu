@@ -835,11 +835,11 @@ router_backward_kernel(const Rows a, const int* __restrict__ routes, const float
   }
 }
 
-// Routes per expert of one sequence by a cluster of eight CTAs: each counts an eighth of the rows in its shared memory
-// and sums a share of the experts over all eight.  Nothing has to be cleared before, so it is one launch: 3.5 us for
-// 8192 x 8 routes to 256 experts, which is little more than a launch.
+// Routes per expert of one sequence by a cluster of eight CTAs: each counts an eighth of the rows in its shared memory,
+// and the first sums each expert over all eight, a thread an expert.  Nothing has to be cleared before, so it is one
+// launch: 3.5 us for 8192 x 8 routes to 256 experts, which is little more than a launch.
 constexpr int kCountCtas = 8;
-__global__ void __cluster_dims__(kCountCtas, 1, 1) __launch_bounds__(1024)
+__global__ void __cluster_dims__(kCountCtas, 1, 1) __launch_bounds__(kMaxExperts)
 expert_counts_cluster_kernel(const Rows a, const int* __restrict__ routes, int* __restrict__ counts) {
   extern __shared__ int cluster_counts[];
   for (int e = threadIdx.x; e < a.experts; e += blockDim.x) cluster_counts[e] = 0;
@@ -854,7 +854,8 @@ expert_counts_cluster_kernel(const Rows a, const int* __restrict__ routes, int* 
     if (static_cast<unsigned>(e) < static_cast<unsigned>(a.experts)) atomicAdd(cluster_counts + e, 1);
   }
   cluster_sync_all();
-  for (int e = part * blockDim.x + threadIdx.x; e < a.experts; e += kCountCtas * blockDim.x) {
+  const int e = threadIdx.x;
+  if (part == 0 && e < a.experts) {
     const uint32_t at = smem_u32(cluster_counts + e);
     int c = 0;
 #pragma unroll
@@ -1126,7 +1127,7 @@ extern "C" int wm_expert_counts(const int32_t* routes, int32_t tokens, int32_t t
   a.sequences = sequences;
   a.num_sequences = rows;
   if (rows <= kClusterSequences && static_cast<long long>(tokens) * top_k <= kClusterRoutes) {
-    expert_counts_cluster_kernel<<<dim3(kCountCtas, rows), 1024, experts * 4, stream>>>(a, routes, counts);
+    expert_counts_cluster_kernel<<<dim3(kCountCtas, rows), kMaxExperts, experts * 4, stream>>>(a, routes, counts);
     count_launch();
     WM_CUDA(cudaGetLastError());
     return WM_OK;
