@@ -627,7 +627,8 @@ router_forward_kernel(const Rows a, int* __restrict__ routes, float* __restrict_
 // block to finish sums the blocks' parts of the loss in their order.  Bound by latency: 13 us for 1171 + 16 records of
 // 512 experts (4.9 MB), a chain of loads, sums and the last block's join.
 // table: [num_sequences][experts] of (f - 1) / n_b, the loss's slope by p up to a constant (p sums to one, so a
-// constant drops out of the gradient; without it the differences near f = 1 keep their digits), then 1 / live sequences.
+// constant drops out of the gradient; without it, taken off before f is rounded, the differences near f = 1 keep their
+// digits), then 1 / live sequences.
 __global__ void __launch_bounds__(kFinishWarps * 32)
 balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ given, int* __restrict__ counts,
                       float* __restrict__ table, float* parts, float* __restrict__ loss) {
@@ -678,10 +679,10 @@ balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ g
     if (given != nullptr) c = e < a.experts ? given[static_cast<long long>(b) * a.experts + e] : 0;
     float part = 0.0f;
     if (e < a.experts) {
-      const float f = all > 0 ? static_cast<float>(static_cast<double>(c) * a.experts / static_cast<double>(all)) : 0.0f;
+      const double f = all > 0 ? static_cast<double>(c) * a.experts / static_cast<double>(all) : 0.0;
       const float inv = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
-      part = n > 0 ? f * (sum / static_cast<float>(n)) : 0.0f;
-      table[static_cast<long long>(b) * a.experts + e] = (f - 1.0f) * inv;
+      part = n > 0 ? static_cast<float>(f) * (sum / static_cast<float>(n)) : 0.0f;
+      table[static_cast<long long>(b) * a.experts + e] = static_cast<float>(f - 1.0) * inv;
       if (counts != nullptr) counts[static_cast<long long>(b) * a.experts + e] = c;
     }
     part = warp_sum(part);
