@@ -709,12 +709,13 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_const
 // scale 1.  Each CTA, one of 128 rows x 32 blocks, notes whether it met a scale that is no power of two.  5.5 us alone,
 // nearly all of it latency (1 MB in, 0.3 MB out for 8192 x 4096 scaled by rows); behind a quantiser its start is hidden.
 __global__ void __launch_bounds__(256)
-pack_scales_kernel(const float* __restrict__ p_scales, int p_rows, int p_shift, uint32_t* __restrict__ p_out,
-                   const float* __restrict__ q_scales, int q_rows, int q_shift, uint32_t* __restrict__ q_out, int kblocks,
-                   int* __restrict__ findings) {
+pack_scales_kernel(const float* p_scales, int p_rows, int p_shift, uint32_t* p_out, const float* q_scales, int q_rows,
+                   int q_shift, uint32_t* q_out, int kblocks, int* findings) {
   __shared__ unsigned char codes[kPackBlocks][128 + 4];
   cudaTriggerProgrammaticLaunchCompletion();   // the product may take its place; it waits for these before it reads
-  cudaGridDependencySynchronize();             // as this kernel does for the one that quantised the operands
+  // As this kernel does for the one that quantised the operands.  That one may still write the scales while this one runs,
+  // so they are read by ordinary loads: no __ldg and no __restrict__ here.
+  cudaGridDependencySynchronize();
   const int p_tiles = (p_rows + 127) / 128;
   const bool of_p = static_cast<int>(blockIdx.x) < p_tiles;
   const int tile = of_p ? blockIdx.x : blockIdx.x - p_tiles;
@@ -729,7 +730,7 @@ pack_scales_kernel(const float* __restrict__ p_scales, int p_rows, int p_shift, 
   for (int i = 0; i < kEach; ++i) {
     const int row = tile * 128 + r0 + i * (256 / kPackBlocks);
     bits[i] = kb < count && row < rows
-                  ? __float_as_uint(__ldg(scales + static_cast<long long>(row >> shift) * kblocks + kb0 + kb)) : 0x3f800000u;
+                  ? __float_as_uint(scales[static_cast<long long>(row >> shift) * kblocks + kb0 + kb]) : 0x3f800000u;
   }
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
