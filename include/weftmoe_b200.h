@@ -246,8 +246,9 @@ WM_API int wm_fp8_gemm(const void* aq, const float* as, const void* bq, const fl
  * summed in FP32 on the tensor cores and added times the product of its two scales in FP32.
  * workspace (optional, NULL = none; wm_fp8_matmul_workspace bytes of device memory, 128-byte aligned, free again when
  * the call's kernels are done): large products whose scales are all powers of two are then scaled on the tensor cores and
- * summed there over up to 32 blocks, which is faster (and cuts instead of rounding: 1.4e-6 of a sum of positive
- * products, 2.2e-7 of one of normal operands); the scales are looked at on the device.
+ * summed there over up to 32 blocks, which is faster but cuts instead of rounding.  Relative errors of an FP32 out, norm
+ * over norm, with / without workspace, at K = 8190: normal operands 2.2e-7 / 1.0e-7, scales that vary by 2^6 between
+ * blocks 5.4e-7 / 1.3e-7; 1.4e-6 / 2.5e-7 where all products are positive.  The scales are looked at on the device.
  * out: rows ld >= n elements apart, BF16 (rounded once) or FP32; accumulate adds into an FP32 out.  k == 0 gives zeros.
  * wm_fp8_matmul_status synchronises `stream`, reads and clears the device's word: *code = WM_ERR_TIMEOUT when a
  * bounded wait of an earlier call ran out (that call's out is then incomplete). */
@@ -323,7 +324,9 @@ WM_API int wm_scatter_output(const void* output, int32_t tokens, int32_t start, 
  * sum, whatever its logits hold.  A live token with a NaN (for softmax also +inf) logit gets the routes
  * 0..top_k-1 with NaN gates, and NaN gradients.
  * Balance loss: mean over the sequences that have a live token of sum_e f_e P_e; f_e = experts * counts_e / sum of
- * counts, P_e = mean over live tokens of score_e / (sum of the token's scores).  Its gradient takes counts as given.
+ * counts, P_e = mean over live tokens of score_e / (sum of the token's scores).  A live token without an available expert
+ * (all logits -inf) has no scores and is left out of both means.  Its gradient takes counts as given.
+ * Scores, gates and sums are FP32; scores below 2^-126 are 0 (shares and renormalised gates of such sigmoids are not).
  * Results do not depend on the order in which blocks run.  No call synchronises or allocates; all may be captured.
  * tokens < 2^26, experts <= 1024, top_k <= 32, num_sequences <= 65535. */
 typedef struct wm_router {

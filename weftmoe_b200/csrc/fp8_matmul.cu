@@ -20,18 +20,19 @@
 // (kind::mxf8f6f4.block_scale, scales as UE8M0 in TMEM) and accumulate up to 32 blocks before the adding warps take them
 // over.  The accumulator cuts what it cannot hold, so its error grows with the number of blocks (normal operands: 4.9e-7
 // of the result at K = 8192 and 3.0e-6 at 32768 in one go); with 32 it stays at 2.2e-7 from K = 4096 up (general form: 0.7
-// to 2.3e-7 from 4096 to 32768), and at 1.4e-6 where all products are positive and every cut goes the same way (general
-// form 0.9 to 2.5e-7).  E4M3 itself is off by up to 2^-4 an operand.  A kernel in front packs the scales and notes
-// whether one is no power of two; the product then takes the general form above.
+// to 2.3e-7 from 4096 to 32768), at 5.4e-7 where the products of scales vary by 2^6 from block to block (general form
+// 1.3e-7, K = 8190), and at 1.4e-6 where all products are positive and every cut goes the same way (general form 0.9 to
+// 2.5e-7).  E4M3 itself is off by up to 2^-4 an operand.  A kernel in front packs the scales and notes whether one is no
+// power of two; the product then takes the general form above.
 // Otherwise `split` CTAs of a cluster may share one tile, each a range of the blocks; their sums are joined through
 // distributed shared memory in a fixed order.
 //
-// What bounds it.  Few rows (64 x 4096 x 4096: 11.5 us; its 17 MB of weights take 2.7 us to read): the start of the
-// kernel, 8 blocks a CTA one after the other, and the join of four sums.  Large products with packed scales (8192 x
-// 4096 x 4096: 97 us, 2.8 PFLOP/s, tensor pipe 76 % busy): operands from shared memory and L2; repeated for seconds
-// the power limit makes it 116 us.  Long K on few tiles (4096 x 2048, K = 8190: 57 us, 60 % busy): 128 tiles on 74 pairs,
-// a second wave that is three quarters full.  General scales on pairs (147 and 154 us for these two): the adding warps, 128
-// accumulators a thread read, scaled and added for every block.
+// What bounds it.  Few rows (64 x 4096 x 4096: 9.3 us back to back; its 17 MB of weights take 2.7 us to read): the start of
+// the kernel, 8 blocks a CTA one after the other, and the join of four sums.  Large products with packed scales (8192 x
+// 4096 x 4096: 94 us on its own with the packing in front, 2.9 PFLOP/s, tensor pipe 76 % busy): operands from shared
+// memory and L2; back to back the power limit makes it 116 us.  Long K on few tiles (4096 x 2048, K = 8190: 58 us replayed,
+// 60 % busy): 128 tiles on 74 pairs, a second wave that is three quarters full, and the packing.  General scales on pairs
+// (137 and 148 us for these two): the adding warps, 128 accumulators a thread read, scaled and added for every block.
 #include <limits.h>
 
 #include <algorithm>

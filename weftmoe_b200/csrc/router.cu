@@ -12,9 +12,10 @@
 // Sums over rows are taken per block in a fixed order into records, and the records in a fixed order by a
 // second kernel, so results do not depend on the order in which blocks run.
 //
-// What bounds it: instructions, not bytes.  A score costs an exponential, an addition and a reciprocal, the choice about as
-// much again; 65536 rows of 512 BF16 logits (67 MB; 10 us at the copy rate) take 76 us for the choice by logits, 98 us
-// by sigmoid + bias, 123 us with the loss on top, at two thirds of the issue slots and 24 warps an SM.
+// What bounds it: instructions and their latency, not bytes.  A score costs an exponential, an addition and a reciprocal,
+// the choice about as much again; 65536 rows of 512 BF16 logits (67 MB; 10 us at the copy rate) take 76 us for the choice by
+// logits, 98 us by sigmoid + bias, 123 us with the loss on top.  Two thirds of the issue slots are taken; the other third is
+// the wait for shuffles, shared memory and spilled registers, which 24 warps an SM do not cover.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -31,7 +32,10 @@ constexpr int kWarps = 8;
 constexpr int kFinishWarps = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTokens = (1 << 26) - 1;   // x 32 routes: counts fit in 32 bits
-constexpr int kMaxBlocks = 1184;  // 148 SMs x 8
+// Records of the loss are one a block, so blocks are limited: 148 SMs x 8.  (512 experts have 444 places, so 2.6 rounds;
+// other limits were not measured.)  A warp then adds the shares of up to tokens / 9472 rows one after another in FP32:
+// 256 at 2.4 M tokens, 7086 at the most tokens there may be.
+constexpr int kMaxBlocks = 1184;
 constexpr int kFewChoices = 12;     // see choose
 template <bool MANY>
 constexpr int kCandidates = MANY ? 64 : 32;   // of one row, for its choice
@@ -500,8 +504,11 @@ struct Records {
   unsigned* ticket;
 };
 
-// Blocks of an SM that the registers are shared out for.  Forward and backward of 65536 rows of 512 experts took 211 us
-// with 3 blocks (80 registers, a few spilled), 213 us with 2 for the backward kernel (no spills), 18 us more with 4.
+// Blocks of an SM that the registers are shared out for.  Forward and backward of 65536 rows of 512 BF16 experts took 211 us
+// with 3 blocks, 213 us with 2 for the backward kernel, 18 us more with 4; the other sizes were not measured.  Limits
+// of 64 and 80 registers spill.  Forward kernels, bytes of spill stores a thread with vector loads and up to 12 choices,
+// BF16 / FP32: 32 experts 60 / 60, 64: 88 / 112, 128: 116 / 156, 256: 216 / 178, 512: 104 / 316, 1024: none.  Backward
+// kernels: 256 experts 0 / 8, 512: 112 / 168, the others none.
 template <int V>
 constexpr int kResident = V <= 8 ? 4 : V <= 16 ? 3 : 1;
 
@@ -722,8 +729,8 @@ balance_finish_kernel(const Rows a, const Records rec, const int* __restrict__ g
 //     sigmoid, renormalised  (1 - s_k) w_k (g_k - sum w g)           sigmoid  (1 - s_k) s_k g_k
 //   loss, q = the table's row times dloss / live sequences:  p_e (q_e - sum p q), times 1 - s_e for sigmoid.
 // The choices' part goes through a row of shared memory that is zero between rows.  A warp takes a.chunk rows in a row, and
-// fetches the next one's logits, routes and dgates ahead.  Bound by instructions (62 % of the issue slots): 85 us under
-// ncu for 65536 rows of 512 BF16 logits, 134 MB in and out, which a copy moves in 20 us.
+// fetches the next one's logits, routes and dgates ahead.  Bound by instructions and their latency (62 % of the issue slots
+// taken): 85 us under ncu for 65536 rows of 512 BF16 logits, 134 MB in and out, which a copy moves in 20 us.
 template <class T, int V, int VEC>
 __global__ void __launch_bounds__(kWarps * 32, kResident<V>)
 router_backward_kernel(const Rows a, const int* __restrict__ routes, const float* __restrict__ dgates,

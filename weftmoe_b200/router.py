@@ -109,8 +109,8 @@ def balance_loss(logits, counts, *, score="softmax", padding_mask=None, sequence
     """The balance loss of a batch, a float32 scalar that is differentiable by the logits.
 
     With p the token's scores as shares of their sum, P_e the mean of p_e over the live tokens and
-    f_e = experts * counts_e / sum(counts): sum over experts of f_e P_e; with `sequences` (int32 offsets,
-    non-decreasing) the mean of that over the sequences that have a live token, counts then being [sequences, experts].
+    f_e = experts * counts_e / sum(counts): sum over experts of f_e P_e (tokens without an available expert are left out);
+    with `sequences` (int32 offsets, non-decreasing) the mean of that over the sequences that have a live token, counts then being [sequences, experts].
     counts come from `expert_counts`, possibly summed over ranks; they are taken as constants.  An even load gives 1."""
     _check_logits(logits)
     _check_score(score)
