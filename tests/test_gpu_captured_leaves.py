@@ -1,5 +1,5 @@
-"""GPU: what a capture may find of its leaves.  A leaf's gradient is accumulated on the stream of the graph that first
-took it; the legacy default stream cannot join a capture, so a forward pass that would lead there is refused."""
+"""GPU: what a captured backward pass may find behind it.  A leaf's gradient is accumulated on the stream of the graph that
+first took it; the legacy default stream cannot join a capture, so gradients that would go there are refused."""
 import pytest
 import torch
 
@@ -26,18 +26,21 @@ def cases():
 
 
 @pytest.mark.parametrize("name", NAMES)
-def test_a_leaf_of_a_live_eager_graph_is_refused_in_a_capture(name):
+def test_gradients_of_a_live_eager_graph_are_refused_in_a_capture(name):
     forward, leaves = cases()[name]
     alive = forward()
     want = torch.autograd.grad(alive, leaves, torch.ones_like(alive), retain_graph=True)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        torch.zeros(1, device="cuda")
-        with pytest.raises(RuntimeError, match="eager graph"):
-            forward()
-        with torch.no_grad():
-            forward()                                             # nothing accumulates behind this
-    del graph, alive
+        y = forward()                                             # a forward pass alone is no trouble
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            y.backward(torch.ones_like(y))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive) and all(leaf.grad is None for leaf in leaves)
+    del graph, alive, y
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         y = forward()
@@ -47,21 +50,35 @@ def test_a_leaf_of_a_live_eager_graph_is_refused_in_a_capture(name):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_gradients_that_do_not_go_there_are_captured():
+    """The weight is a leaf of a live eager graph, but the captured gradient is the input's alone."""
+    g = torch.Generator("cuda").manual_seed(95)
+    weight = torch.randn(96, 256, device="cuda", dtype=torch.bfloat16, generator=g, requires_grad=True)
+    prepared = prepare_fp8_linear(weight)
+    x = torch.randn(40, 256, device="cuda", dtype=torch.bfloat16, generator=g)
+    alive = fp8_linear(x, weight, prepared)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = x.clone().requires_grad_()
+        y = fp8_linear(inside, weight, prepared)
+        dx, = torch.autograd.grad(y, inside, torch.ones_like(y))
+    graph.replay()
+    torch.cuda.synchronize()
+    outside = x.clone().requires_grad_()
+    assert torch.equal(y, alive)
+    assert torch.equal(dx, torch.autograd.grad(fp8_linear(outside, weight, prepared), outside, torch.ones_like(y))[0])
+
+
 @pytest.mark.parametrize("name", NAMES)
-def test_other_live_graphs_are_no_reason(name):
-    """Eager calls beside each other, and a live graph of a side stream, which could join."""
+def test_eager_backward_passes_beside_other_streams_are_as_before(name):
     forward, leaves = cases()[name]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         alive = forward()
+        there = torch.autograd.grad(alive, leaves, torch.ones_like(alive), retain_graph=True)
     torch.cuda.current_stream().wait_stream(side)
-    again = forward()
-    assert torch.equal(alive, again)
-    del again
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        inside = forward()
-    graph.replay()
-    torch.cuda.synchronize()
-    assert torch.equal(inside, alive)
+    here = forward()
+    assert torch.equal(alive, here)
+    got = torch.autograd.grad(here, leaves, torch.ones_like(here))
+    assert all(torch.equal(a, b) for a, b in zip(got, there))

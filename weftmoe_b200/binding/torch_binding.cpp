@@ -47,6 +47,26 @@ void refuse_tangent(const char* what, const Tensor& t) {
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, " has no derivative in forward mode");
 }
 
+// In a backward pass under capture: gradients that go on to a node of the legacy default stream, as to a leaf whose
+// gradient an eager graph, still alive, accumulates there.  That stream cannot join a capture; autograd would have it wait
+// for this one, which fails and can take the process along, so this is refused before anything is enqueued.
+void refuse_uncaptured_gradient(const char* what, const Tensor& like) {
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const c10::Stream outside = c10::cuda::getDefaultCUDAStream(like.device().index()).unwrap();
+  for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+    const torch::autograd::Edge& edge = node->next_edge(i);
+    if (!edge.is_valid() || !node->task_should_compute_output(i)) continue;
+    const optional<c10::Stream> stream = edge.function->stream();
+    if (!stream.has_value() || *stream != outside) continue;
+    const c10::cuda::CUDAGuard guard(like.device());
+    TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None, what,
+                " cannot be captured: one goes to a leaf or a node of an eager graph on the default stream; drop that "
+                "graph before the capture, or make it on a side stream");
+    return;
+  }
+}
+
 template <class T>
 T* data(const Tensor& t) {
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
@@ -139,6 +159,7 @@ Tensor router_backward(const Tensor& rows, const Choice& c, const Tensor& paddin
   refuse_second_derivative("The router's gradients");
   const bool gates_part = dgates.defined(), loss_part = dloss.defined();
   if (!gates_part && !loss_part) return Tensor();
+  refuse_uncaptured_gradient("The router's gradients", rows);
   Launch launch(rows);
   if (gates_part) dgates = dgates.to(at::kFloat).contiguous();   // broadcast gradients are expanded
   if (loss_part) dloss = dloss.to(at::kFloat).contiguous();
@@ -212,26 +233,10 @@ struct Balance : torch::autograd::Function<Balance> {
 
 bool wants_gradient(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
-// In a capture: a leaf whose gradient an eager graph, still alive, accumulates on the legacy default stream.  That stream
-// cannot join a capture, and the captured backward pass, which would have to wait for it, fails inside autograd and can
-// take the process along; so the forward pass is refused.
-void refuse_eager_leaf(const char* what, const Tensor& t) {
-  if (!t.is_cuda() || !wants_gradient(t) || !t.is_leaf()) return;
-  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!held) return;
-  const optional<c10::Stream> stream = held->stream();
-  if (!stream.has_value() || *stream != c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap()) return;
-  const c10::cuda::CUDAGuard guard(t.device());
-  TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None, what,
-              ": an eager graph of this leaf on the default stream is alive; drop its results before a capture, or make "
-              "them on a side stream");
-}
-
 variable_list route(const Tensor& logits, int64_t top_k, int64_t score, bool renormalize, double scale,
                     const optional<Tensor>& bias, const optional<Tensor>& padding, const optional<Tensor>& sequences,
                     bool balance) {
   refuse_tangent("The router", logits);
-  refuse_eager_leaf("The router", logits);
   const Choice c{top_k, score, renormalize, scale};
   if (wants_gradient(logits))
     return Route::apply(logits, c, bias, padding, sequences, balance);
@@ -243,7 +248,6 @@ variable_list route(const Tensor& logits, int64_t top_k, int64_t score, bool ren
 Tensor balance(const Tensor& logits, const Tensor& counts, int64_t score, const optional<Tensor>& padding,
                const optional<Tensor>& sequences) {
   refuse_tangent("balance_loss", logits);
-  refuse_eager_leaf("balance_loss", logits);
   if (wants_gradient(logits)) return Balance::apply(logits, counts, score, padding, sequences);
   return balance_forward(rows_of(logits), counts, score, or_none(padding), or_none(sequences)).first;
 }
@@ -362,6 +366,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const variable_list s = ctx->get_saved_variables();
     variable_list out(7);
     if (!grads[0].defined()) return out;
+    refuse_uncaptured_gradient("The gradients of fp8_linear", grads[0]);
     const Tensor& weight = s[0];
     const Tensor dy = grads[0].contiguous();
     const bool to_x = ctx->needs_input_grad(0), to_weight = ctx->needs_input_grad(1);
@@ -389,8 +394,6 @@ Tensor fp8_linear(const Tensor& x, const Tensor& weight, const Tensor& wq, const
   refuse_tangent("fp8_linear", x);
   refuse_tangent("fp8_linear", weight);
   check_sizes({x.size(0), x.size(1), weight.size(0)});
-  refuse_eager_leaf("fp8_linear", x);
-  refuse_eager_leaf("fp8_linear", weight);
   const bool to_weight = wants_gradient(weight);
   if (wants_gradient(x) || to_weight) return Linear::apply(x, weight, wq, ws, wtq, wts, to_weight);
   return linear_forward(x, wq, ws, weight.size(0));
