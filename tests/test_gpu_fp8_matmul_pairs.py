@@ -60,3 +60,14 @@ def test_packed_scales_of_128_rows_on_the_left(m, n, k, a_rows, b_rows, dtype):
     a, b = operand(m, k, a_rows, 62), operand(n, k, b_rows, 63)
     assert torch.equal(fp8_matmul(a, b, dtype=dtype), (wide(a) @ wide(b).t()).float().to(dtype))
     poll_fp8_matmul()
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("m, n, pitch", [(130, 517, 520), (130, 65, 72), (300, 1001, 1008), (1500, 1701, 1704), (4100, 4199, 4200)])
+def test_results_of_odd_width_in_aligned_rows(m, n, pitch, dtype):
+    """Rows that start on 16 bytes and end between: what lies behind them stays."""
+    a, b = operand(m, 640, 1, 64), operand(n, 640, 128, 65)
+    holder = torch.full((m, pitch), 7.0, dtype=dtype, device="cuda")
+    fp8_matmul(a, b, dtype=dtype, out=holder[:, :n])
+    assert torch.equal(holder[:, :n], (wide(a) @ wide(b).t()).float().to(dtype))
+    assert (holder[:, n:] == 7).all()

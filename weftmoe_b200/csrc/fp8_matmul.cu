@@ -273,8 +273,8 @@ __device__ __forceinline__ void store_row(const MatmulArgs& a, int p, int q, con
     if (q + j < a.q_rows) store_one<false>(a, p, q + j, v[j]);
 }
 // A warp's 32 rows x 2 * PAIRS columns by way of shared memory: boxes of 32 rows x 128 bytes, 16-byte pieces swizzled by
-// the row.  From there TMA writes them (tma_store; the map clips what lies outside the matrix), or, where the rows of out are
-// not aligned or are added to, the warp does, row by row: 64 or 128 neighbouring bytes an instruction.
+// the row.  From there TMA writes them (tma_store; the map clips what lies outside the matrix), or, where the rows of out do
+// not start and end on 16 bytes or are added to, the warp does, row by row: 64 or 128 neighbouring bytes an instruction.
 template <int PAIRS>
 __device__ __forceinline__ void store_boxes(const MatmulArgs& a, const CUtensorMap* tmap, uint8_t* staging, int p, int q,
                                             int lane, const uint64_t (&sum)[PAIRS]) {
@@ -918,7 +918,8 @@ extern "C" int wm_fp8_matmul(const void* aq, const float* as, const void* bq, co
   if (int rc = make_tmap_2d(&tp, swap ? bq : aq, 1, k, a.p_rows, pitch, 128, 128)) return rc;
   if (int rc = make_tmap_2d(&tq, swap ? aq : bq, 1, k, a.q_rows, pitch, 128, bn)) return rc;
   CUtensorMap tout = tp;   // not read without tma_store
-  a.tma_store = !swap && a.vector_store && !accumulate;
+  // A TMA store writes 16 bytes at a time, also where the map's rows end between: those would reach behind column n.
+  a.tma_store = !swap && a.vector_store && !accumulate && static_cast<long long>(n) * element % 16 == 0;
   if (a.tma_store)
     if (int rc = make_tmap_2d(&tout, out, element, n, m, static_cast<uint64_t>(ld) * element, 128 / element, 32)) return rc;
   CUtensorMap tsp = tp, tsq = tp;   // not read without packed scales
